@@ -51,6 +51,12 @@ SIGNATURES = {
     "dscq_pack_int4": [_P, _I64, _I64, _P, _P],
     "dscq_pack_int4_checked": [_P, _I, _I64, _I64, _P, _P, _P],
     "dscq_unpack_int4": [_P, _I64, _I64, _I64, _P, _P],
+    "dscq_kv_append": [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I, _I64, _I64, _I64, _I64,
+                       _P, _P, _P, _I64, _I64, _I, _I, _P, _P, _I64, _I64, _P, _P],
+    "dscq_kv_read": [_P, _I64, _I64, _I64, _I64, _P, _I64, _I, _I, _P, _P, _P],
+    "dscq_kv_attention_workspace_bytes": [_I64, _I64, _I64, _I64, _I64, _I64, _I64],
+    "dscq_kv_attention": [_P, _I64, _I64, _I, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64, _P,
+                          _P, _I64, _I64, _I64, _F, _I64, _P, _P, _P, _I64, _P],
     "dscq_time_next_kernel": [_P, _P],
     "dscq_set_gemm_kernel": [_I],
     "dscq_stream_probe": [_P, _I64, _P, _I64, _I, _P],
@@ -83,6 +89,7 @@ def lib() -> ctypes.CDLL:
             L.dscq_matmul_workspace_bytes.restype = ctypes.c_int64
             L.dscq_linear_workspace_bytes.restype = ctypes.c_int64
             L.dscq_gated_mlp_workspace_bytes.restype = ctypes.c_int64
+            L.dscq_kv_attention_workspace_bytes.restype = ctypes.c_int64
             _lib = L
     return _lib
 

@@ -354,6 +354,81 @@ int64_t dscq_gated_mlp_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t 
 int dscq_device_supported(void);
 
 /*
+ * The 4-bit paged key/value cache of an attention layer: appending to it, reading it
+ * back, attending over it.  No reference counterpart exists (its decoder runs attention
+ * in torch, core/model_ops.py:18-29); rows are quantized by the rule of activation_codes
+ * at 4 bits (core/quantization.py:13-21), the zero-point kept in the scale's last bits.
+ *
+ * cache  u8 [pages, H, page_size, D + 8], 16-byte aligned: page_size a multiple of 16 up
+ *   to 4096, H key/value heads (up to 1024), D = 64 or 128.  The bytes of one (page, head):
+ *     keys    [page_size/16][4][16][D/32] 32-bit words: token 16 a + r, elements g D/4 + 8 w
+ *             to + 7 are word [a][g][r][w], in its nibbles 0 4 1 5 2 6 3 7 (from the lowest)
+ *     values  [page_size/4][16][2][D/64] words: token 4 a + 2 b + h, element c D/16 + 4 m + j
+ *             is nibble 4 h + j of word [a][c][b][m]
+ *     words   [page_size] of the keys, then [page_size] of the values: the scale as fp32,
+ *             its last four bits the zero-point
+ *   A row x of D numbers: lo = min(x, 0), hi = max(x, 0), base = max((hi - lo) / 15, 1e-8)
+ *   rounded up to a multiple of 16 last places, zero = round(-lo / base) in [0, 15],
+ *   scale = base + zero last places, code = round(x / scale + zero) in [0, 15], standing for
+ *   (code - zero) * scale; all in fp32.  A row that is not finite is stored as NaN.
+ * slot   page * page_size + place of a token; slots of one call are distinct.
+ *
+ * dscq_kv_append: the step's rows into their slots.
+ *   q, k, v    rows of T tokens, fp16 or bf16 (dtype), the D elements of a head contiguous,
+ *              tokens and heads at the given strides (elements); q NULL: none.
+ *   cos, sin   f32 [table_rows, rotary / 2] (rotary a multiple of 16 up to D), or NULL: the
+ *              first `rotary` elements of each head of q and k are turned by row
+ *              positions[t], in fp32: pairs (i, i + rotary / 2), or (2 i, 2 i + 1) where
+ *              `interleaved`.
+ *   rotate     1: keys are stored as H_D k (unnormalised Sylvester Hadamard), queries
+ *              returned as H_D q / D, so that scores are unchanged and the outliers of a few
+ *              channels are spread over the row before it is quantized.
+ *   slots      a slot outside the cache: the token is not stored.  A position outside the
+ *              table: not stored either, and its queries are NaN.
+ *   q_out      [T, Hq, D] of the rows' type.
+ */
+int dscq_kv_append(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                   int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                   int64_t v_token_stride, int64_t v_head_stride, int dtype, int64_t T, int64_t Hq,
+                   int64_t H, int64_t D, const int64_t* positions, const float* cos,
+                   const float* sin, int64_t table_rows, int64_t rotary, int interleaved,
+                   int rotate, const int64_t* slots, uint8_t* cache, int64_t pages,
+                   int64_t page_size, void* q_out, void* stream);
+
+/* Cached tokens as rows: k, v out [T, H, D] fp16 or bf16, in the basis they were appended
+ * in (rotate as in dscq_kv_append); a slot outside the cache gives zeros. */
+int dscq_kv_read(const uint8_t* cache, int64_t pages, int64_t page_size, int64_t H, int64_t D,
+                 const int64_t* slots, int64_t T, int rotate, int dtype, void* k, void* v,
+                 void* stream);
+
+/*
+ * Causal attention of a ragged batch over the cache: sequence b's queries are rows
+ * starts[b] .. starts[b + 1] - 1 of q, the last of its lengths[b] cached tokens; the query
+ * at place p sees the tokens j <= p (and j > p - window where window > 0).
+ *   out = softmax(scale q k^T) v, keys and values as the exact numbers they are stored as,
+ *   scores, maximum, sum and products in fp32.  A query that sees no token: out 0, lse -inf.
+ *   q        [T, Hq, D] fp16 or bf16 at the given strides; query head h reads cache head
+ *            h / (Hq / H).
+ *   tables   i32 [B, width]: the pages of each sequence, in order; tokens of a page outside
+ *            the cache are not seen.
+ *   lengths  i32 [B]; at most width * page_size tokens are seen.
+ *   starts   i32 [B + 1], or NULL: one query a sequence (T = B, max_q = 1).
+ *   max_q, max_length  bounds of a sequence's queries and length known to the host: queries
+ *            past max_q are not computed; longer lengths are, less evenly.
+ *   out      [T, Hq, D] of q's type; lse f32 [T, Hq] (natural logarithm) or NULL.
+ *   workspace  16-byte aligned scratch of dscq_kv_attention_workspace_bytes (may be 0).
+ * Limits: Hq a multiple of H up to 4096, B <= 65535, scale > 0.
+ */
+int64_t dscq_kv_attention_workspace_bytes(int64_t B, int64_t Hq, int64_t H, int64_t D,
+                                          int64_t max_q, int64_t max_length, int64_t window);
+int dscq_kv_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype,
+                      int64_t T, int64_t Hq, const uint8_t* cache, int64_t pages,
+                      int64_t page_size, int64_t H, int64_t D, const int32_t* tables,
+                      int64_t width, const int32_t* lengths, const int32_t* starts, int64_t B,
+                      int64_t max_q, int64_t max_length, float scale, int64_t window, void* out,
+                      float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * Kernel timing without a profiler (no reference counterpart): the next call
  * the calling thread makes into this library stamps the device start and end
  * times of its kernel into the HIP events `start` and `stop` (hipEvent_t created
