@@ -23,6 +23,7 @@
 namespace dscq {
 
 constexpr int kKvTile = 16;      // tokens of a key tile; pages are whole tiles
+constexpr int64_t kKvMaxLength = int64_t{1} << 28;  // tokens of a sequence
 constexpr uint32_t kKvNan = 0x7FC00000u;  // the word of a row that is not finite
 
 struct KvCache {

@@ -36,7 +36,6 @@ int check_dtype(int dtype) {
 
 // Tokens of one call: their workgroups fit a grid, their rows 64-bit offsets.
 constexpr int64_t kMaxTokens = int64_t{1} << 30;
-constexpr int64_t kMaxLength = int64_t{1} << 28;  // of a sequence
 
 int check_attention(int64_t B, int64_t Hq, int64_t heads, int64_t D, int64_t max_q,
                     int64_t max_length, int64_t window) {
@@ -136,7 +135,7 @@ int dscq_kv_attention(const void* q, int64_t q_token_stride, int64_t q_head_stri
   if (int rc = check_dtype(dtype)) return rc;
   if (int rc = check_cache(cache, pages, page_size, H, D)) return rc;
   if (int rc = check_attention(B, Hq, H, D, max_q, max_length, window)) return rc;
-  if (!(T >= 0 && T <= kMaxTokens && width >= 0 && width <= kMaxLength / page_size))
+  if (!(T >= 0 && T <= kMaxTokens && width >= 0 && width <= kKvMaxLength / page_size))
     return fail("kv attention: invalid dimensions");
   if (!(scale > 0.0f && scale < 3.0e38f)) return fail("kv attention: scale must be positive");
   if (T == 0 || B == 0 || max_q == 0) return DSCQ_OK;

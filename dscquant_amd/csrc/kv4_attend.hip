@@ -28,69 +28,17 @@
 
 #include <algorithm>
 
-#include "kv4.h"
-#include "mma_int4.h"
-#include "rowquant.h"
+#include "kv4_attend.h"
 
 namespace dscq {
 
+int kv_attend_prompt(const KvAttend& a, int D, bool is_bf16, const Part& part, int waves,
+                     int chunks, int least, hipStream_t stream);
+
 namespace {
 
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef float f4 __attribute__((ext_vector_type(4)));
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kWaves = 4;
 constexpr int kStep = 2 * kKvTile;  // tokens of a step
-
-// A value every lane holds alike, read through the scalar cache.
-__device__ __forceinline__ int32_t uniform_load(const int32_t* p) {
-  typedef const __attribute__((address_space(4))) int32_t* Ptr;
-  return *(Ptr)(reinterpret_cast<uintptr_t>(p));
-}
-
-// Sequence b's queries (rows first .. first + n - 1 of q) and length.
-struct Sequence {
-  int64_t first;
-  int n, L;
-};
-__device__ __forceinline__ Sequence sequence_of(const KvAttend& a, int b) {
-  int64_t s0 = b, s1 = b + 1;
-  if (a.starts) {
-    s0 = max(uniform_load(a.starts + b), 0);
-    s1 = uniform_load(a.starts + b + 1);
-  }
-  s0 = min(s0, a.T);
-  s1 = min(max(s1, s0), a.T);
-  const int64_t L = min((int64_t)max(uniform_load(a.lengths + b), 0), a.width * a.cache.P);
-  return {s0, (int)min(s1 - s0, (int64_t)a.max_q), (int)L};
-}
-
-// One past the last token that query i sees, and the first.
-__device__ __forceinline__ int row_end(const Sequence& s, int i) { return max(s.L - s.n + i + 1, 0); }
-__device__ __forceinline__ int row_begin(const KvAttend& a, const Sequence& s, int i) {
-  const int64_t b = (int64_t)(s.L - s.n + i + 1) - a.window;
-  return a.window && b > 0 ? (int)b : 0;
-}
-
-template <int D>
-struct Words {  // a lane's D/8 bytes of a tile
-  uint32_t w[D / 32];
-};
-template <int D>
-__device__ __forceinline__ Words<D> load_words(const uint8_t* p) {
-  Words<D> r;
-  if constexpr (D == 128) {
-    const uint4 x = *reinterpret_cast<const uint4*>(p);
-    r.w[0] = x.x; r.w[1] = x.y; r.w[2] = x.z; r.w[3] = x.w;
-  } else {
-    const uint2 x = *reinterpret_cast<const uint2*>(p);
-    r.w[0] = x.x; r.w[1] = x.y;
-  }
-  return r;
-}
 
 // What a lane reads of a 16-token tile.
 template <int D>
@@ -101,66 +49,29 @@ struct Tile {
   bool there;    // uniform: the tile's page is one of the cache
 };
 
+// A tile's address is a uniform one (its page's block and place) and a lane's offset that
+// never changes, the two addends of a global load.
 template <int D>
 struct Pages {
+  Places places;
   const uint8_t* head;  // the head's block of page 0
-  const int32_t* table;
   int64_t page_bytes, pages;
-  int P, per, end;      // tokens and tiles of a page; one past the last token
-  uint32_t inverse;     // ceil(2^32 / per)
+  uint32_t k_at, v_at, kz_at, kf_at, vf_at;  // the lane's
 };
 
 template <int D>
-__device__ __forceinline__ int page_index(const Pages<D>& g, int tile) {
-  return g.per == 1 ? tile : (int)__umulhi((uint32_t)tile, g.inverse);
-}
-// The table's entry for a tile, -1 past the end.
-template <int D>
-__device__ __forceinline__ int page_of(const Pages<D>& g, int tile) {
-  return tile * kKvTile < g.end ? uniform_load(g.table + page_index(g, tile)) : -1;
-}
-
-template <int D>
-__device__ __forceinline__ Tile<D> load_tile(const Pages<D>& g, int tile, int page, int lane) {
+__device__ __forceinline__ Tile<D> load_tile(const Pages<D>& g, Place p) {
   Tile<D> t;
-  t.there = page >= 0 && page < g.pages;
-  const int at = t.there ? (tile - page_index(g, tile) * g.per) * kKvTile : 0;
-  const uint8_t* block = g.head + (int64_t)(t.there ? page : 0) * g.page_bytes;
-  t.k = load_words<D>(block + at * (D / 2) + lane * (D / 8));
-  t.v = load_words<D>(block + (g.P + at) * (D / 2) + lane * (D / 8));
-  const uint8_t* words = block + g.P * D + at * 4;
-  t.kz = *reinterpret_cast<const uint32_t*>(words + (lane & 15) * 4);
-  t.kf = *reinterpret_cast<const uint4*>(words + (lane >> 4) * 16);
-  t.vf = *reinterpret_cast<const uint4*>(words + g.P * 4 + (lane >> 4) * 16);
+  t.there = p.page >= 0 && p.page < g.pages;
+  const uint8_t* block = g.head + (t.there ? p.page * g.page_bytes : 0);
+  const uint8_t* codes = block + p.at * (8 * D);
+  const uint8_t* words = block + p.at * (4 * kKvTile);
+  t.k = load_words<D>(codes + g.k_at);
+  t.v = load_words<D>(codes + g.v_at);
+  t.kz = *reinterpret_cast<const uint32_t*>(words + g.kz_at);
+  t.kf = *reinterpret_cast<const uint4*>(words + g.kf_at);
+  t.vf = *reinterpret_cast<const uint4*>(words + g.vf_at);
   return t;
-}
-
-// Two nibbles 16 bits apart as fp16 numbers less their zero-points.  0x6400 | c is the
-// fp16 number 1024 + c; with the nibble four bits up, 1024 + 16 c, a sixteenth of which is
-// 64 + c.  Both subtractions are exact.
-struct ZeroPair {
-  h2 low, high;  // -(1024 + z), -(64 + z)
-};
-__device__ __forceinline__ ZeroPair zero_pair(uint32_t word0, uint32_t word1) {
-  // Bytes 0 of the two words, 16 bits apart (the bytes between are masked off).
-  const uint32_t z = __builtin_amdgcn_perm(word1, word0, 0x0C040C00u);
-  ZeroPair r;
-  r.low = __builtin_bit_cast(h2, (z & 0x000F000Fu) | 0xE400E400u);
-  r.high = __builtin_bit_cast(h2, ((z << 4) & 0x00F000F0u) | 0xD400D400u);
-  return r;
-}
-__device__ __forceinline__ void unpack_word(uint32_t w, const ZeroPair& z, h2 out[4]) {
-  const h2 sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t x = w >> (8 * i);
-    out[2 * i] = __builtin_bit_cast(h2, (x & 0x000F000Fu) | 0x64006400u) + z.low;
-    out[2 * i + 1] = __builtin_elementwise_fma(
-        __builtin_bit_cast(h2, (x & 0x00F000F0u) | 0x64006400u), sixteenth, z.high);
-  }
-}
-__device__ __forceinline__ h8 join8(h2 a, h2 b, h2 c, h2 d) {
-  return (h8){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
 __device__ __forceinline__ float xor16(float v) { return __shfl_xor(v, 16); }
@@ -225,15 +136,16 @@ struct Rows {
   __device__ __forceinline__ void step(const Tile<D>& a, const Tile<D>& b, int j0, int lane,
                                        bool whole) {
     const int g4 = (lane >> 4) * 4;
+    const Masks masks;
     h8 kk[2][D / 32];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const Tile<D>& t = h ? b : a;
-      const ZeroPair z = zero_pair(t.kz, t.kz);
+      const ZeroPair z = zero_pair(t.kz, t.kz, masks);
 #pragma unroll
       for (int w = 0; w < D / 32; ++w) {
         h2 e[4];
-        unpack_word(t.k.w[w], z, e);
+        unpack_word(t.k.w[w], z, masks, e);
         kk[h][w] = join8(e[0], e[1], e[2], e[3]);
       }
     }
@@ -329,15 +241,15 @@ struct Rows {
 #pragma unroll
       for (int i = 0; i < 8; ++i) p[r][i] = (_Float16)e[i];
     }
-    const ZeroPair z[4] = {zero_pair(a.vf.x, a.vf.y), zero_pair(a.vf.z, a.vf.w),
-                           zero_pair(b.vf.x, b.vf.y), zero_pair(b.vf.z, b.vf.w)};
+    const ZeroPair z[4] = {zero_pair(a.vf.x, a.vf.y, masks), zero_pair(a.vf.z, a.vf.w, masks),
+                           zero_pair(b.vf.x, b.vf.y, masks), zero_pair(b.vf.z, b.vf.w, masks)};
 #pragma unroll
     for (int w = 0; w < D / 64; ++w) {
       h2 e[4][4];
-      unpack_word(a.v.w[w], z[0], e[0]);
-      unpack_word(a.v.w[D / 64 + w], z[1], e[1]);
-      unpack_word(b.v.w[w], z[2], e[2]);
-      unpack_word(b.v.w[D / 64 + w], z[3], e[3]);
+      unpack_word(a.v.w[w], z[0], masks, e[0]);
+      unpack_word(a.v.w[D / 64 + w], z[1], masks, e[1]);
+      unpack_word(b.v.w[w], z[2], masks, e[2]);
+      unpack_word(b.v.w[D / 64 + w], z[3], masks, e[3]);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const h8 v = join8(e[0][t], e[1][t], e[2][t], e[3][t]);
@@ -364,15 +276,15 @@ struct Rows {
     }
     lo = __builtin_amdgcn_readfirstlane(lo);
     hi = __builtin_amdgcn_readfirstlane(hi);
-    Tile<D> a = load_tile<D>(g, 2 * first, page_of(g, 2 * first), lane);
-    Tile<D> b = load_tile<D>(g, 2 * first + 1, page_of(g, 2 * first + 1), lane);
-    int pa = page_of(g, 2 * (first + stride)), pb = page_of(g, 2 * (first + stride) + 1);
+    Tile<D> a = load_tile<D>(g, place_of(g.places, 2 * first));
+    Tile<D> b = load_tile<D>(g, place_of(g.places, 2 * first + 1));
+    Place pa = place_of(g.places, 2 * (first + stride)), pb = place_of(g.places, 2 * (first + stride) + 1);
     for (int st = first; st < last; st += stride) {
       const int next = st + stride;
-      const Tile<D> na = load_tile<D>(g, 2 * next, pa, lane);
-      const Tile<D> nb = load_tile<D>(g, 2 * next + 1, pb, lane);
-      pa = page_of(g, 2 * (next + stride));
-      pb = page_of(g, 2 * (next + stride) + 1);
+      const Tile<D> na = load_tile<D>(g, pa);
+      const Tile<D> nb = load_tile<D>(g, pb);
+      pa = place_of(g.places, 2 * (next + stride));
+      pb = place_of(g.places, 2 * (next + stride) + 1);
       step(a, b, st * kStep, lane,
            st * kStep >= lo && st * kStep + kStep <= hi && a.there && b.there);
       a = na;
@@ -381,29 +293,42 @@ struct Rows {
   }
 };
 
-// The launch's plan; `chunks` > 1: the tokens are split over that many workgroups and the
-// parts joined by a second kernel.
+// The launch's plan.  Rows go in groups of `rows`, their tokens in up to `chunks` parts of
+// whole steps of `step` tokens, at least `least` of them each; groups of more than one part
+// are joined by a second kernel (launched where chunks > 1).
 struct Plan {
-  int rt, chunks;
-  bool rows;  // the waves of a workgroup take different rows, not different tokens
+  int rows, step, chunks, least;
+  bool prompt;  // kv4_prompt.hip
 };
 
-struct Part {  // a row's result over some of its tokens
-  float* out;  // [rows][chunks][D], rows = (b max_q + i) Hq + head
-  float* log;  // [rows][chunks]: log2 of the softmax sum
+// The steps of a group's tokens and of each part, and how many parts it has.
+struct Parts {
+  int first, last, each, used;
 };
+__device__ __forceinline__ Parts parts_of(const KvAttend& a, const Sequence& s, const Plan& p, int G,
+                                          int r0) {
+  const int r1 = min(r0 + p.rows, s.n * G) - 1;
+  Parts x;
+  x.first = row_begin(a, s, r0 / G) / p.step;
+  x.last = (row_end(s, r1 / G) + p.step - 1) / p.step;
+  x.each = max((x.last - x.first + p.chunks - 1) / p.chunks, p.least);
+  x.used = max((x.last - x.first + x.each - 1) / x.each, 1);
+  return x;
+}
 
 template <int D>
-__device__ __forceinline__ Pages<D> pages_of(const KvAttend& a, int b, int h, int end) {
+__device__ __forceinline__ Pages<D> pages_of(const KvAttend& a, int b, int h, int end, int lane) {
   Pages<D> g;
-  g.P = a.cache.P;
-  g.per = g.P / kKvTile;
-  g.inverse = (uint32_t)((0x100000000ull + g.per - 1) / g.per);
-  g.page_bytes = a.cache.H * kv_block_bytes<D>(g.P);
-  g.head = a.cache.data + h * kv_block_bytes<D>(g.P);
+  const int P = a.cache.P;
+  g.places = places_of(a, b, end);
+  g.page_bytes = a.cache.H * kv_block_bytes<D>(P);
+  g.head = a.cache.data + h * kv_block_bytes<D>(P);
   g.pages = a.cache.pages;
-  g.table = a.tables + b * a.width;
-  g.end = end;
+  g.k_at = lane * (D / 8);
+  g.v_at = P * (D / 2) + lane * (D / 8);
+  g.kz_at = P * D + (lane & 15) * 4;
+  g.kf_at = P * D + (lane >> 4) * 16;
+  g.vf_at = P * (D + 4) + (lane >> 4) * 16;
   return g;
 }
 
@@ -433,29 +358,27 @@ __device__ __forceinline__ float log_sum(const Rows<D, RT>& rows, int r, float l
              : __builtin_amdgcn_logf(l) + rows.m[r] * rows.to2[r] - rows.x;
 }
 
-// Grid: (chunks, H * row tiles, B); the four waves of a workgroup take every fourth step of
-// its tokens and join their results through LDS.
+// Grid: (chunks, H, B), up to 16 RT rows; the four waves of a workgroup take every fourth
+// step of its tokens and join their results through LDS.
 template <int D, typename T, int RT>
-__global__ __launch_bounds__(64 * kWaves) void kv_attend_split_kernel(KvAttend a, Part part,
-                                                                      int row_tiles) {
+__global__ __launch_bounds__(64 * kWaves, RT == 1 ? 3 : 1) void kv_attend_split_kernel(
+    KvAttend a, Part part, Plan plan) {
   constexpr int kRow = D + 4;
   __shared__ float out[kWaves][16][kRow];
   __shared__ float logs[kWaves][16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int b = blockIdx.z, h = blockIdx.y / row_tiles, tile = blockIdx.y - h * row_tiles;
-  const int G = a.Hq / a.cache.H, r0 = tile * 16 * RT, chunks = gridDim.x;
+  const int b = blockIdx.z, h = blockIdx.y;
+  const int G = a.Hq / a.cache.H;
   const Sequence s = sequence_of(a, b);
   const int count = s.n * G;
-  if (r0 >= count) return;
-  const int i0 = r0 / G, i1 = min(r0 + 16 * RT, count) - 1;
-  const int first = row_begin(a, s, i0) / kStep;
-  const int last = (row_end(s, i1 / G) + kStep - 1) / kStep;
-  const int each = max((last - first + chunks - 1) / chunks, 1);
-  const int from = first + blockIdx.x * each, to = min(from + each, last);
-  if (blockIdx.x > 0 && from >= last) return;
+  if (count == 0) return;
+  const Parts parts = parts_of(a, s, plan, G, 0);
+  if ((int)blockIdx.x >= parts.used) return;
+  const int from = parts.first + blockIdx.x * parts.each;
+  const int to = min(from + parts.each, parts.last);
   Rows<D, RT> rows;
-  begin_rows<D, T, RT>(rows, a, s, h, G, r0, lane);
-  const Pages<D> pages = pages_of<D>(a, b, h, row_end(s, i1 / G));
+  begin_rows<D, T, RT>(rows, a, s, h, G, 0, lane);
+  const Pages<D> pages = pages_of<D>(a, b, h, row_end(s, s.n - 1), lane);
   rows.run(pages, from + wave, to, kWaves, lane);
   const int c = lane & 15, g = lane >> 4;
 #pragma unroll
@@ -471,7 +394,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attend_split_kernel(KvAttend a
     if (g == 0) logs[wave][c] = log_sum(rows, r, l);
     __syncthreads();
     const int row = threadIdx.x >> 4, d = (threadIdx.x & 15) * (D / 16);
-    const int R = r0 + 16 * r + row;
+    const int R = 16 * r + row;
     if (R < count) {
       float top = logs[0][row];
 #pragma unroll
@@ -488,8 +411,8 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attend_split_kernel(KvAttend a
       const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
       const float log = sum == 0.0f ? -INFINITY : base + __builtin_amdgcn_logf(sum);
       const int i = R / G, hq = h * G + R - i * G;
-      if (chunks > 1) {
-        const int64_t at = (((int64_t)b * a.max_q + i) * a.Hq + hq) * chunks + blockIdx.x;
+      if (parts.used > 1) {
+        const int64_t at = (((int64_t)b * a.max_q + i) * a.Hq + hq) * plan.chunks + blockIdx.x;
 #pragma unroll
         for (int e = 0; e < D / 16; ++e) part.out[at * D + d + e] = y[e] * scale;
         if (d == 0) part.log[at] = log;
@@ -505,130 +428,133 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attend_split_kernel(KvAttend a
   }
 }
 
-// Grid: (max_q Hq, B), a wave a row: its parts weighted by their sums.
+// Grid: (max_q Hq, B): a row's parts weighted by their sums.  The four waves of a workgroup
+// take every fourth part, eight at a time so that their loads are in flight together.
 template <int D, typename T>
-__global__ __launch_bounds__(64) void kv_attend_join_kernel(KvAttend a, Part part, int chunks,
-                                                            int rt) {
-  const int lane = threadIdx.x, b = blockIdx.y, i = blockIdx.x / a.Hq, hq = blockIdx.x - i * a.Hq;
+__global__ __launch_bounds__(64 * kWaves) void kv_attend_join_kernel(
+    KvAttend a, Part part, Plan plan, int per) {
+  __shared__ float out[kWaves][D], sums[kWaves];
+  const int lane = threadIdx.x & 63;
+  // This wave's share of its row: every `per`-th part.
+  int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int b = blockIdx.y;
+  const int row = blockIdx.x * (kWaves / per) + wave / per, i = row / a.Hq, hq = row - i * a.Hq;
+  wave %= per;
   const Sequence s = sequence_of(a, b);
-  if (i >= s.n) return;
-  // How many parts the row's workgroup made: as kv_attend_split_kernel.
-  const int G = a.Hq / a.cache.H, count = s.n * G;
-  const int r0 = (i * G + hq % G) / (16 * rt) * (16 * rt);
-  const int first = row_begin(a, s, r0 / G) / kStep;
-  const int last = (row_end(s, (min(r0 + 16 * rt, count) - 1) / G) + kStep - 1) / kStep;
-  const int each = max((last - first + chunks - 1) / chunks, 1);
-  const int used = max((last - first + each - 1) / each, 1);
+  const int G = a.Hq / a.cache.H, chunks = plan.chunks;
+  int used = 0;
+  if (i < s.n) used = parts_of(a, s, plan, G, (i * G + hq % G) / plan.rows * plan.rows).used;
+  const bool in = used > 1;  // a row of one part is done
+  if (per == kWaves && !in) return;
   const int64_t at = (((int64_t)b * a.max_q + i) * a.Hq + hq) * chunks;
   float top = -INFINITY;
   for (int c = lane; c < used; c += 64) top = fmaxf(top, part.log[at + c]);
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
   const float base = top == -INFINITY ? 0.0f : top;
-  float sum = 0.0f, y[D / 64] = {};
-  for (int c = 0; c < used; ++c) {
-    const float p = __builtin_amdgcn_exp2f(part.log[at + c] - base);
-    sum += p;
+  constexpr int kE = D / 64, kMany = 8;
+  float sum = 0.0f, y[kE] = {};
+  for (int c = wave; in && c < used; c += kMany * per) {
+    float log[kMany], x[kMany][kE];
 #pragma unroll
-    for (int e = 0; e < D / 64; ++e)
-      y[e] = __builtin_fmaf(p, part.out[(at + c) * D + lane * (D / 64) + e], y[e]);
+    for (int m = 0; m < kMany; ++m) {
+      const int64_t from = at + min(c + m * per, used - 1);
+      log[m] = part.log[from];
+#pragma unroll
+      for (int e = 0; e < kE; ++e) x[m][e] = part.out[from * D + lane * kE + e];
+    }
+#pragma unroll
+    for (int m = 0; m < kMany; ++m) {
+      const float p = c + m * per < used ? __builtin_amdgcn_exp2f(log[m] - base) : 0.0f;
+      sum += p;
+#pragma unroll
+      for (int e = 0; e < kE; ++e) y[e] = p == 0.0f ? y[e] : __builtin_fmaf(p, x[m][e], y[e]);
+    }
   }
-  const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
-  const int64_t to = (s.first + i) * a.Hq + hq;
-  uint16_t* o = static_cast<uint16_t*>(a.out) + to * D + lane * (D / 64);
+  if (per > 1) {
+    const int w = threadIdx.x >> 6;
 #pragma unroll
-  for (int e = 0; e < D / 64; ++e) o[e] = __builtin_bit_cast(uint16_t, to_out<T>(y[e] * scale));
+    for (int e = 0; e < kE; ++e) out[w][lane * kE + e] = y[e];
+    if (lane == 0) sums[w] = sum;
+    __syncthreads();
+    if (wave) return;
+    for (int o = 1; o < per; ++o) {
+      sum += sums[w + o];
+#pragma unroll
+      for (int e = 0; e < kE; ++e) y[e] += out[w + o][lane * kE + e];
+    }
+  }
+  if (!in) return;
+  const int64_t to = (s.first + i) * a.Hq + hq;
+  uint16_t* o = static_cast<uint16_t*>(a.out) + to * D + lane * kE;
+#pragma unroll
+  for (int e = 0; e < kE; ++e)
+    o[e] = __builtin_bit_cast(uint16_t, to_out<T>(sum == 0.0f ? 0.0f : y[e] / sum));
   if (a.lse && lane == 0)
     a.lse[to] = sum == 0.0f ? -INFINITY : (base + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
-// Grid: (H * row tiles / 4, B): a wave takes 64 rows over all their tokens.
-template <int D, typename T, int RT>
-__global__ __launch_bounds__(64 * kWaves) void kv_attend_rows_kernel(KvAttend a, int row_tiles) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int b = blockIdx.y, groups = (row_tiles + kWaves - 1) / kWaves;
-  const int h = blockIdx.x % a.cache.H;
-  const int tile = (groups - 1 - blockIdx.x / a.cache.H) * kWaves + wave;
-  const int G = a.Hq / a.cache.H, r0 = tile * 16 * RT;
-  const Sequence s = sequence_of(a, b);
-  const int count = s.n * G;
-  if (r0 >= count) return;
-  const int i0 = r0 / G, i1 = (min(r0 + 16 * RT, count) - 1) / G;
-  Rows<D, RT> rows;
-  begin_rows<D, T, RT>(rows, a, s, h, G, r0, lane);
-  const int end = row_end(s, i1);
-  const Pages<D> pages = pages_of<D>(a, b, h, end);
-  rows.run(pages, row_begin(a, s, i0) / kStep, (end + kStep - 1) / kStep, 1, lane);
-  const int c = lane & 15, g = lane >> 4;
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    const int row = r0 + 16 * r + c, i = row / G;
-    const float l = row_sum(rows.l[r]);
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    if (row < count) {
-      const int64_t at = (s.first + i) * a.Hq + h * G + row - i * G;
-      uint16_t* o = static_cast<uint16_t*>(a.out) + at * D + g * (D / 4);
-#pragma unroll
-      for (int e = 0; e < D / 4; e += 8) {
-        u32x4_a2 w;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int d = e + 2 * x;
-          w[x] = pack_pair<T>(rows.o[r][d % (D / 16)][d / (D / 16)] * inv,
-                              rows.o[r][(d + 1) % (D / 16)][d / (D / 16)] * inv);
-        }
-        *reinterpret_cast<u32x4_a2*>(o + e) = w;
-      }
-      if (a.lse && g == 0) a.lse[at] = log_sum(rows, r, l) * kLn2;
-    }
-  }
-}
-
 Plan plan_of(int B, int Hq, int H, int max_q, int64_t max_length, int64_t window) {
-  const int64_t rows = (int64_t)max_q * (Hq / H);
-  Plan p = {4, 1, rows > 64};
-  if (p.rows) return p;
-  p.rt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  int64_t length = window ? std::min(max_length, window + max_q - 1) : max_length;
-  const int64_t most = (length + kWaves * kStep - 1) / (kWaves * kStep);
-  const int64_t want = (3 * (int64_t)cu_count() + B * H - 1) / (B * H);
-  p.chunks = (int)std::max<int64_t>(1, std::min(most, want));
+  const int64_t rows = (int64_t)max_q * (Hq / H), cus = cu_count();
+  const int64_t length =
+      std::min<int64_t>(window ? std::min(max_length, window + max_q - 1) : max_length, kKvMaxLength);
+  Plan p = {};
+  int64_t groups = 1, slots;
+  if (rows > 64) {
+    // 256 rows a workgroup, one of which a CU holds, or 128 (two).
+    p.prompt = true;
+    p.rows = rows > 128 ? 256 : 128;
+    p.step = p.rows / 2;
+    p.least = 2;
+    groups = (rows + p.rows - 1) / p.rows;
+    slots = cus * (256 / p.rows);
+  } else {
+    // As many workgroups as the device holds at once: each has the same tokens to read, so
+    // a second round would only add its start and end (131072 tokens of 8 heads: 36 us in
+    // one round, 41 in two, 49 in four).
+    p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+    p.step = kStep;
+    p.least = kWaves;
+    slots = cus * (p.rows == 16 ? 3 : 1);
+  }
+  const int64_t steps = (length + p.step - 1) / p.step + 1, wgs = groups * B * H;
+  const int64_t want = p.prompt ? slots / wgs : (slots + wgs - 1) / wgs;
+  p.chunks = (int)std::max<int64_t>(1, std::min((steps + p.least - 1) / p.least, want));
+  p.least = (int)std::max<int64_t>(p.least, (steps + p.chunks - 1) / p.chunks);
   return p;
-}
-
-template <int D, typename T, int RT>
-int attend_split(const KvAttend& a, const Plan& p, void* ws, hipStream_t stream) {
-  const int rows = a.max_q * (a.Hq / a.cache.H), tiles = (rows + 16 * RT - 1) / (16 * RT);
-  Part part = {nullptr, nullptr};
-  if (p.chunks > 1) {
-    part.out = static_cast<float*>(ws);
-    part.log = part.out + (int64_t)a.B * a.max_q * a.Hq * p.chunks * D;
-  }
-  const KernelEvents ev = take_kernel_events();
-  arm_kernel_events({ev.start, p.chunks > 1 ? nullptr : ev.stop});
-  launch(kv_attend_split_kernel<D, T, RT>, dim3(p.chunks, a.cache.H * tiles, a.B),
-         dim3(64 * kWaves), stream, a, part, tiles);
-  if (p.chunks > 1) {
-    arm_kernel_events({nullptr, ev.stop});
-    launch(kv_attend_join_kernel<D, T>, dim3(a.max_q * a.Hq, a.B), dim3(64), stream, a, part,
-           p.chunks, RT);
-  }
-  return launch_status("kv_attention");
 }
 
 template <int D, typename T>
 int attend(const KvAttend& a, void* ws, hipStream_t stream) {
   const Plan p = plan_of(a.B, a.Hq, a.cache.H, a.max_q, a.max_length, a.window);
-  if (p.rows) {
-    const int64_t rows = (int64_t)a.max_q * (a.Hq / a.cache.H), tiles = (rows + 63) / 64;
-    launch(kv_attend_rows_kernel<D, T, 4>,
-           dim3((uint32_t)((tiles + kWaves - 1) / kWaves * a.cache.H), a.B), dim3(64 * kWaves),
-           stream, a, (int)tiles);
-    return launch_status("kv_attention");
+  Part part = {nullptr, nullptr};
+  if (p.chunks > 1) {
+    part.out = static_cast<float*>(ws);
+    part.log = part.out + (int64_t)a.B * a.max_q * a.Hq * p.chunks * D;
   }
-  if (p.rt == 1) return attend_split<D, T, 1>(a, p, ws, stream);
-  if (p.rt == 2) return attend_split<D, T, 2>(a, p, ws, stream);
-  return attend_split<D, T, 4>(a, p, ws, stream);
+  // Timing events, if armed, span both kernels.
+  const KernelEvents ev = take_kernel_events();
+  arm_kernel_events({ev.start, p.chunks > 1 ? nullptr : ev.stop});
+  const dim3 grid(p.chunks, a.cache.H, a.B), block(64 * kWaves);
+  int rc = 0;
+  if (p.prompt)
+    rc = kv_attend_prompt(a, D, std::is_same<T, bf16>::value, part, p.rows / 32, p.chunks, p.least,
+                          stream);
+  else if (p.rows == 16)
+    launch(kv_attend_split_kernel<D, T, 1>, grid, block, stream, a, part, p);
+  else if (p.rows == 32)
+    launch(kv_attend_split_kernel<D, T, 2>, grid, block, stream, a, part, p);
+  else
+    launch(kv_attend_split_kernel<D, T, 4>, grid, block, stream, a, part, p);
+  if (rc) return rc;
+  if (p.chunks > 1) {
+    // A row's parts by one wave, or, where there are many, by four.
+    const int per = p.chunks <= 16 ? 1 : kWaves, rows = kWaves / per;
+    arm_kernel_events({nullptr, ev.stop});
+    launch(kv_attend_join_kernel<D, T>, dim3((a.max_q * a.Hq + rows - 1) / rows, a.B), block, stream,
+           a, part, p, per);
+  }
+  return launch_status("kv_attention");
 }
 
 }  // namespace
