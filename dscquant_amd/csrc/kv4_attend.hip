@@ -39,6 +39,7 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kStep = 2 * kKvTile;  // tokens of a step
+constexpr int kAhead = 2;           // steps whose codes are on their way
 
 // What a lane reads of a 16-token tile.
 template <int D>
@@ -86,160 +87,128 @@ __device__ __forceinline__ float row_sum(float v) {
   return v + xor32(v);
 }
 
-// A lane's quarter of one row of q: elements g D/4 .. + D/4 - 1, as fp16 times 2^k; k.
-template <int D, typename T>
-__device__ __forceinline__ int load_q(const T* row, bool in, int g, h8 q[D / 32]) {
-  float x[D / 32][8];
-  float top = 0.0f;
-#pragma unroll
-  for (int w = 0; w < D / 32; ++w) {
-    to_f32(load_raw_at<T>(row, (uint32_t)(in ? g * (D / 4) + 8 * w : 0)), x[w]);
-    mask_f32<T>(in, x[w]);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[w][e]));
-  }
-  int k = 0;
-  if constexpr (std::is_same<T, bf16>::value) {
-    top = row_max(top);
-    if (top > 0.0f && top < INFINITY) k = 15 - __builtin_amdgcn_frexp_expf(top);
-  }
-#pragma unroll
-  for (int w = 0; w < D / 32; ++w)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) q[w][e] = (_Float16)__builtin_amdgcn_ldexpf(x[w][e], k);
-  return k;
-}
-
-// The running state of RT tiles of sixteen rows in one wave; lane (c, g) holds row c's
-// statistics (l: of its own tokens) and its elements g D/4 .. + D/4 - 1 of the output.
-template <int D, int RT>
+// The running state of sixteen rows in one wave; lane (c, g) holds row c's statistics (l: of
+// its own tokens) and its elements g D/4 .. + D/4 - 1 of the output.
+template <int D>
 struct Rows {
-  h8 q[RT][D / 32];
-  f4 o[RT][D / 16];  // o[r][t][i]: element (4 g + i) D/16 + t
-  float to2[RT];     // scores to binary places: scale log2 e 2^-k
-  float m[RT], off[RT], limit[RT], l[RT];  // maximum; x - m to2; what moves the maximum
-  int begin[RT], end[RT];                  // the row's tokens
-  float x, value_limit;                    // the values' exponent, the scale that moves it
+  h8 q[D / 32];
+  f4 o[D / 16];                                   // o[t][i]: element (4 g + i) D/16 + t
+  float off = 0.0f, limit = -INFINITY, l = 0.0f;  // x less the maximum; what moves it; the sum
+  float x = 0.0f, value_limit = 0.0f;             // the values' exponent, the scale that moves it
+  float to2;                                      // scores to binary places: scale log2 e 2^-k
+  int begin, end, all_begin, all_end;             // the row's tokens; those that every row sees
 
-  __device__ __forceinline__ void clear() {
+  // The rows of a sequence and key/value head h: their q, and what they see.
+  template <typename T>
+  __device__ __forceinline__ void load(const KvAttend& a, const Sequence& s, int h, int G, int lane) {
+    // A row past the last one is the last one over again; it is not stored.
+    const int g = lane >> 4, row = min(lane & 15, s.n * G - 1), i = row / G;
+    const T* p = static_cast<const T*>(a.q) + (s.first + i) * a.q_ts + (h * G + row - i * G) * a.q_hs;
+    Raw<T> raw[D / 32];
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
+    for (int w = 0; w < D / 32; ++w) raw[w] = load_raw_at<T>(p, g * (D / 4) + 8 * w);
 #pragma unroll
-      for (int t = 0; t < D / 16; ++t) o[r][t] = (f4){0, 0, 0, 0};
-      m[r] = limit[r] = -INFINITY;
-      off[r] = l[r] = 0.0f;
-    }
-    x = value_limit = 0.0f;
-  }
-
-  // The 32 tokens from j0 in tiles a and b; `whole`: every row sees them all.
-  __device__ __forceinline__ void step(const Tile<D>& a, const Tile<D>& b, int j0, int lane,
-                                       bool whole) {
-    const int g4 = (lane >> 4) * 4;
-    const Masks masks;
-    h8 kk[2][D / 32];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const Tile<D>& t = h ? b : a;
-      const ZeroPair z = zero_pair(t.kz, t.kz, masks);
+    for (int t = 0; t < D / 16; ++t) o[t] = (f4){0, 0, 0, 0};
+    begin = row_begin(a, s, i);
+    end = row_end(s, i);
+    all_begin = row_begin(a, s, s.n - 1);
+    all_end = row_end(s, 0);
+    int k = 0;
+    if constexpr (std::is_same<T, bf16>::value) {
+      float top = 0.0f, y[8];
 #pragma unroll
       for (int w = 0; w < D / 32; ++w) {
-        h2 e[4];
-        unpack_word(t.k.w[w], z, masks, e);
-        kk[h][w] = join8(e[0], e[1], e[2], e[3]);
+        to_f32(raw[w], y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(y[e]));
       }
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+      if (top > 0.0f && top < INFINITY) k = min(15 - __builtin_amdgcn_frexp_expf(top), 60);
     }
+    to2 = __builtin_amdgcn_ldexpf(a.scale * kLog2e, -k);
+#pragma unroll
+    for (int w = 0; w < D / 32; ++w) {
+      float y[8];
+      to_f32(raw[w], y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) q[w][e] = (_Float16)__builtin_amdgcn_ldexpf(y[e], k);
+    }
+  }
+
+  // The 32 tokens from j0 in tiles a and b.
+  __device__ __forceinline__ void step(const Tile<D>& a, const Tile<D>& b, int j0, int lane,
+                                       const Masks& masks) {
     float vf[8] = {__uint_as_float(a.vf.x), __uint_as_float(a.vf.y), __uint_as_float(a.vf.z),
                    __uint_as_float(a.vf.w), __uint_as_float(b.vf.x), __uint_as_float(b.vf.y),
                    __uint_as_float(b.vf.z), __uint_as_float(b.vf.w)};
     const float kf[8] = {__uint_as_float(a.kf.x), __uint_as_float(a.kf.y), __uint_as_float(a.kf.z),
                          __uint_as_float(a.kf.w), __uint_as_float(b.kf.x), __uint_as_float(b.kf.y),
                          __uint_as_float(b.kf.z), __uint_as_float(b.kf.w)};
-    float s[RT][8];
+    float s[8];
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      f4 c0 = {0, 0, 0, 0}, c1 = {0, 0, 0, 0};
+    for (int h = 0; h < 2; ++h) {
+      const Tile<D>& t = h ? b : a;
+      const ZeroPair z = zero_pair(t.kz, t.kz, masks);
+      f4 c = {0, 0, 0, 0};
 #pragma unroll
       for (int w = 0; w < D / 32; ++w) {
-        c0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[0][w], q[r][w], c0, 0, 0, 0);
-        c1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[1][w], q[r][w], c1, 0, 0, 0);
+        h2 e[4];
+        unpack_word(t.k.w[w], z, masks, e);
+        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(join8(e[0], e[1], e[2], e[3]), q[w], c, 0, 0, 0);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[r][i] = c0[i] * kf[i];
-        s[r][4 + i] = c1[i] * kf[4 + i];
-      }
+      for (int i = 0; i < 4; ++i) s[4 * h + i] = __builtin_fmaf(c[i], kf[4 * h + i] * to2, off);
+      // One tile's numbers in registers at a time.
+      __builtin_amdgcn_sched_barrier(0);
     }
+    const bool whole = j0 >= all_begin && j0 + kStep <= all_end && a.there && b.there;
     if (!whole) {
       // Tokens a row does not see, and pages that are not there: score -inf, and a scale
       // of 0, for what lies there may be anything.
-      bool none[8];
+      const int g4 = (lane >> 4) * 4;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) none[i] = true;
-#pragma unroll
-      for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int j = j0 + (i < 4 ? g4 + i : 12 + g4 + i);
-          const bool seen = (i < 4 ? a.there : b.there) && j >= begin[r] && j < end[r];
-          s[r][i] = seen ? s[r][i] : -INFINITY;
-          none[i] = none[i] && !seen;
-        }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) vf[i] = none[i] ? 0.0f : vf[i];
+      for (int i = 0; i < 8; ++i) {
+        const int j = j0 + (i < 4 ? g4 + i : 12 + g4 + i);
+        const bool seen = (i < 4 ? a.there : b.there) & (j >= begin) & (j < end);
+        s[i] = seen ? s[i] : -INFINITY;
+        vf[i] = seen ? vf[i] : 0.0f;
+      }
     }
-    float top[RT];
-    bool move = false;
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      top[r] = fmaxf(fmaxf(fmaxf(s[r][0], s[r][1]), fmaxf(s[r][2], s[r][3])),
-                     fmaxf(fmaxf(s[r][4], s[r][5]), fmaxf(s[r][6], s[r][7])));
-      move = move || top[r] > limit[r];
-    }
+    const float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])),
+                            fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
     float most = fmaxf(fmaxf(fmaxf(vf[0], vf[1]), fmaxf(vf[2], vf[3])),
                        fmaxf(fmaxf(vf[4], vf[5]), fmaxf(vf[6], vf[7])));
-    move = move || most > value_limit;
-    if (__builtin_amdgcn_ballot_w64(move)) {
+    if (__builtin_amdgcn_ballot_w64((top > limit) | (most > value_limit))) {
       float shift = 0.0f;
-      // Masked rows can differ in what they see, so the largest scale is the wave's.
+      // Rows can differ in what they see, so the largest scale is the wave's.
 #pragma unroll
       for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
       if (most > value_limit) {
-        const float to = (float)(7 - __builtin_amdgcn_frexp_expf(most));
-        shift = to - x;
-        x = to;
-        value_limit = __builtin_amdgcn_ldexpf(1.0f, 7 - (int)to);
+        const int e = __builtin_amdgcn_frexp_expf(most);
+        shift = (float)(7 - e) - x;
+        x = (float)(7 - e);
+        value_limit = __builtin_amdgcn_ldexpf(1.0f, e);
       }
+      // A row whose largest score passed its limit gets it as the new maximum.
+      const float high = row_max(top);
+      const bool up = high > limit, fresh = limit == -INFINITY;
+      const float delta = up ? x - high : shift;
+      const float keep = fresh ? 0.0f : __builtin_amdgcn_exp2f(delta);
+      limit = up || !fresh ? x + 8.0f : limit;
+      off += delta;
+      l *= keep;
 #pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        const float was = m[r] * to2[r];
-        m[r] = fmaxf(m[r], row_max(top[r]));
-        const float base = m[r] == -INFINITY ? 0.0f : m[r] * to2[r];
-        off[r] = x - base;
-        limit[r] = m[r] + 8.0f / to2[r];
-        const float keep = m[r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(was - base + shift);
-        l[r] *= keep;
+      for (int t = 0; t < D / 16; ++t) o[t] *= keep;
 #pragma unroll
-        for (int t = 0; t < D / 16; ++t) o[r][t] *= keep;
-      }
+      for (int i = 0; i < 8; ++i) s[i] += delta;
     }
-    h8 p[RT];
+    h8 p;
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      float e[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][i], to2[r], off[r]));
-        l[r] += e[i];
-        e[i] *= vf[i];
-      }
-      if (!whole) {
-        // A token that this row does not see may be NaN to another row of the lane.
-#pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = s[r][i] == -INFINITY ? 0.0f : e[i];
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) p[r][i] = (_Float16)e[i];
+    for (int i = 0; i < 8; ++i) {
+      const float e = __builtin_amdgcn_exp2f(s[i]);
+      l += e;
+      p[i] = (_Float16)(e * vf[i]);
     }
     const ZeroPair z[4] = {zero_pair(a.vf.x, a.vf.y, masks), zero_pair(a.vf.z, a.vf.w, masks),
                            zero_pair(b.vf.x, b.vf.y, masks), zero_pair(b.vf.z, b.vf.w, masks)};
@@ -251,70 +220,74 @@ struct Rows {
       unpack_word(b.v.w[w], z[2], masks, e[2]);
       unpack_word(b.v.w[D / 64 + w], z[3], masks, e[3]);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const h8 v = join8(e[0][t], e[1][t], e[2][t], e[3][t]);
+      for (int t = 0; t < 4; ++t)
+        o[4 * w + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+            join8(e[0][t], e[1][t], e[2][t], e[3][t]), p, o[4 * w + t], 0, 0, 0);
+    }
+  }
+
+  // The steps first, first + stride, ... below `last` (tokens / 32).  While one step is
+  // computed the next two steps' codes are on their way, and the one's after them pages.
+  __device__ __forceinline__ void run(const Pages<D>& g, int first, int last, int stride, int lane) {
+    if (first >= last) return;
+    const Masks masks;
+    Tile<D> a[kAhead + 1], b[kAhead + 1];
+    Place pa = place_of(g.places, 2 * first), pb = place_of(g.places, 2 * first + 1);
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
-          o[r][4 * w + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[r], o[r][4 * w + t], 0, 0, 0);
+    for (int i = 0; i < kAhead; ++i) {
+      a[i] = load_tile<D>(g, pa);
+      b[i] = load_tile<D>(g, pb);
+      pa = place_of(g.places, 2 * (first + (i + 1) * stride));
+      pb = place_of(g.places, 2 * (first + (i + 1) * stride) + 1);
+    }
+    for (int st = first;; st += (kAhead + 1) * stride) {
+#pragma unroll
+      for (int i = 0; i <= kAhead; ++i) {
+        const int at = st + i * stride, to = (i + kAhead) % (kAhead + 1);
+        a[to] = load_tile<D>(g, pa);
+        b[to] = load_tile<D>(g, pb);
+        pa = place_of(g.places, 2 * (at + (kAhead + 1) * stride));
+        pb = place_of(g.places, 2 * (at + (kAhead + 1) * stride) + 1);
+        step(a[i], b[i], at * kStep, lane, masks);
+        if (at + stride >= last) return;
       }
     }
   }
-
-  // The steps first, first + stride, ... below `last` (tokens / 32).
-  __device__ __forceinline__ void run(const Pages<D>& g, int first, int last, int stride, int lane) {
-    if (first >= last) return;
-    int lo = 0, hi = 0x7FFFFFFF;  // every row sees the tokens lo .. hi - 1
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      lo = max(lo, begin[r]);
-      hi = min(hi, end[r]);
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      lo = max(lo, __shfl_xor(lo, d));
-      hi = min(hi, __shfl_xor(hi, d));
-    }
-    lo = __builtin_amdgcn_readfirstlane(lo);
-    hi = __builtin_amdgcn_readfirstlane(hi);
-    Tile<D> a = load_tile<D>(g, place_of(g.places, 2 * first));
-    Tile<D> b = load_tile<D>(g, place_of(g.places, 2 * first + 1));
-    Place pa = place_of(g.places, 2 * (first + stride)), pb = place_of(g.places, 2 * (first + stride) + 1);
-    for (int st = first; st < last; st += stride) {
-      const int next = st + stride;
-      const Tile<D> na = load_tile<D>(g, pa);
-      const Tile<D> nb = load_tile<D>(g, pb);
-      pa = place_of(g.places, 2 * (next + stride));
-      pb = place_of(g.places, 2 * (next + stride) + 1);
-      step(a, b, st * kStep, lane,
-           st * kStep >= lo && st * kStep + kStep <= hi && a.there && b.there);
-      a = na;
-      b = nb;
-    }
-  }
 };
 
-// The launch's plan.  Rows go in groups of `rows`, their tokens in up to `chunks` parts of
-// whole steps of `step` tokens, at least `least` of them each; groups of more than one part
-// are joined by a second kernel (launched where chunks > 1).
+// The launch's plan.
+//   kWhole   a workgroup takes all tokens of its rows: grid (1, H, B), one kernel;
+//   kShares  each of `wgs` workgroups a head takes the same share of the batch's steps
+//            (step tokens of one sequence each, in order, at least `least`), whichever
+//            sequences that is; a second kernel joins the parts of a sequence;
+//   kPrompt  kv4_prompt.hip: groups of `rows` rows, their tokens in up to `chunks` parts of
+//            at least `least` steps, joined likewise where chunks > 1.
+enum Form { kWhole, kShares, kPrompt };
 struct Plan {
-  int rows, step, chunks, least;
-  bool prompt;  // kv4_prompt.hip
+  Form form;
+  int rows, waves, step, wgs, chunks, least;
 };
 
-// The steps of a group's tokens and of each part, and how many parts it has.
-struct Parts {
-  int first, last, each, used;
+// The 32-token steps of a sequence's rows: one at least if there are any (empty rows are
+// written too).
+struct Steps {
+  int first, count;
 };
-__device__ __forceinline__ Parts parts_of(const KvAttend& a, const Sequence& s, const Plan& p, int G,
-                                          int r0) {
-  const int r1 = min(r0 + p.rows, s.n * G) - 1;
-  Parts x;
-  x.first = row_begin(a, s, r0 / G) / p.step;
-  x.last = (row_end(s, r1 / G) + p.step - 1) / p.step;
-  x.each = max((x.last - x.first + p.chunks - 1) / p.chunks, p.least);
-  x.used = max((x.last - x.first + x.each - 1) / x.each, 1);
-  return x;
+__device__ __forceinline__ Steps steps_of(const KvAttend& a, const Sequence& s) {
+  if (s.n <= 0) return {0, 0};
+  const int first = row_begin(a, s, 0) / kStep;
+  return {first, max((row_end(s, s.n - 1) + kStep - 1) / kStep - first, 1)};
 }
+
+// Where a sequence's parts are, written by kv_attend_split_kernel for the join: the first
+// one's slot, and how many (1: the rows are done).
+struct Where {
+  int slot, used;
+};
+struct Shares {
+  Part part;     // [slots][H][rows][D]
+  Where* where;  // [B]
+};
 
 template <int D>
 __device__ __forceinline__ Pages<D> pages_of(const KvAttend& a, int b, int h, int end, int lane) {
@@ -332,123 +305,174 @@ __device__ __forceinline__ Pages<D> pages_of(const KvAttend& a, int b, int h, in
   return g;
 }
 
-template <int D, typename T, int RT>
-__device__ __forceinline__ void begin_rows(Rows<D, RT>& rows, const KvAttend& a, const Sequence& s,
-                                           int h, int G, int r0, int lane) {
-  rows.clear();
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    const int row = r0 + 16 * r + (lane & 15), i = row / G;
-    const bool in = i < s.n;
-    const T* p = static_cast<const T*>(a.q) + (s.first + (in ? i : 0)) * a.q_ts +
-                 (h * G + (in ? row - i * G : 0)) * a.q_hs;
-    const int k = load_q<D, T>(p, in, lane >> 4, rows.q[r]);
-    rows.to2[r] = __builtin_amdgcn_ldexpf(a.scale * kLog2e, -k);
-    // A row past the last one sees what the last one does.
-    rows.begin[r] = row_begin(a, s, min(i, s.n - 1));
-    rows.end[r] = row_end(s, min(i, s.n - 1));
-  }
-}
+template <int D, int NW>
+struct Joint {  // LDS in which the waves of a workgroup join their results
+  float out[NW][16][D + 4];
+  float log[NW][16];
+};
 
-// log2 of a row's softmax sum.
-template <int D, int RT>
-__device__ __forceinline__ float log_sum(const Rows<D, RT>& rows, int r, float l) {
-  return rows.m[r] == -INFINITY && l == 0.0f
-             ? -INFINITY
-             : __builtin_amdgcn_logf(l) + rows.m[r] * rows.to2[r] - rows.x;
-}
-
-// Grid: (chunks, H, B), up to 16 RT rows; the four waves of a workgroup take every fourth
-// step of its tokens and join their results through LDS.
-template <int D, typename T, int RT>
-__global__ __launch_bounds__(64 * kWaves, RT == 1 ? 3 : 1) void kv_attend_split_kernel(
-    KvAttend a, Part part, Plan plan) {
-  constexpr int kRow = D + 4;
-  __shared__ float out[kWaves][16][kRow];
-  __shared__ float logs[kWaves][16];
+// Steps from .. to - 1 of sequence b for head h, joined over the waves: the rows' result, or
+// (slot >= 0) their part.
+template <int D, typename T, int NW>
+__device__ __forceinline__ void attend_steps(const KvAttend& a, const Shares& shares,
+                                             Joint<D, NW>& joint, const Sequence& s, int b,
+                                             int h, int from, int to, int64_t slot) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int b = blockIdx.z, h = blockIdx.y;
-  const int G = a.Hq / a.cache.H;
-  const Sequence s = sequence_of(a, b);
-  const int count = s.n * G;
-  if (count == 0) return;
-  const Parts parts = parts_of(a, s, plan, G, 0);
-  if ((int)blockIdx.x >= parts.used) return;
-  const int from = parts.first + blockIdx.x * parts.each;
-  const int to = min(from + parts.each, parts.last);
-  Rows<D, RT> rows;
-  begin_rows<D, T, RT>(rows, a, s, h, G, 0, lane);
+  const int G = a.Hq / a.cache.H, count = s.n * G;
+  Rows<D> rows;
   const Pages<D> pages = pages_of<D>(a, b, h, row_end(s, s.n - 1), lane);
-  rows.run(pages, from + wave, to, kWaves, lane);
+  rows.template load<T>(a, s, h, G, lane);
+  rows.run(pages, from + wave, to, NW, lane);
   const int c = lane & 15, g = lane >> 4;
+  const float l = row_sum(rows.l), inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    if (r) __syncthreads();
-    const float l = row_sum(rows.l[r]);
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int t = 0; t < D / 16; t += 4)
+      *reinterpret_cast<f4*>(&joint.out[wave][c][(4 * g + i) * (D / 16) + t]) =
+          (f4){rows.o[t][i] * inv, rows.o[t + 1][i] * inv, rows.o[t + 2][i] * inv,
+               rows.o[t + 3][i] * inv};
+  if (g == 0) joint.log[wave][c] = l == 0.0f ? -INFINITY : __builtin_amdgcn_logf(l) - rows.off;
+  __syncthreads();
+  // Sixteen lanes a row, D/16 elements each.
+  const int row = threadIdx.x >> 4;
+  if (row < count) {
+    const int d = (threadIdx.x & 15) * (D / 16);
+    float top = joint.log[0][row];
 #pragma unroll
-      for (int t = 0; t < D / 16; ++t)
-        out[wave][c][(4 * g + i) * (D / 16) + t] = rows.o[r][t][i] * inv;
-    if (g == 0) logs[wave][c] = log_sum(rows, r, l);
-    __syncthreads();
-    const int row = threadIdx.x >> 4, d = (threadIdx.x & 15) * (D / 16);
-    const int R = 16 * r + row;
-    if (R < count) {
-      float top = logs[0][row];
+    for (int w = 1; w < NW; ++w) top = fmaxf(top, joint.log[w][row]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f, y[D / 16] = {};
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) top = fmaxf(top, logs[w][row]);
-      const float base = top == -INFINITY ? 0.0f : top;
-      float sum = 0.0f, y[D / 16] = {};
+    for (int w = 0; w < NW; ++w) {
+      const float p = __builtin_amdgcn_exp2f(joint.log[w][row] - base);
+      sum += p;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        const float p = __builtin_amdgcn_exp2f(logs[w][row] - base);
-        sum += p;
+      for (int e = 0; e < D / 16; ++e) y[e] = __builtin_fmaf(p, joint.out[w][row][d + e], y[e]);
+    }
+    const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float log = sum == 0.0f ? -INFINITY : base + __builtin_amdgcn_logf(sum);
+    if (slot >= 0) {
+      const int64_t at = (slot * a.cache.H + h) * ((int64_t)a.max_q * G) + row;
 #pragma unroll
-        for (int e = 0; e < D / 16; ++e) y[e] = __builtin_fmaf(p, out[w][row][d + e], y[e]);
-      }
-      const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
-      const float log = sum == 0.0f ? -INFINITY : base + __builtin_amdgcn_logf(sum);
-      const int i = R / G, hq = h * G + R - i * G;
-      if (parts.used > 1) {
-        const int64_t at = (((int64_t)b * a.max_q + i) * a.Hq + hq) * plan.chunks + blockIdx.x;
+      for (int e = 0; e < D / 16; ++e) shares.part.out[at * D + d + e] = y[e] * scale;
+      if (d == 0) shares.part.log[at] = log;
+    } else {
+      const int i = row / G;
+      const int64_t at = (s.first + i) * a.Hq + h * G + row - i * G;
+      uint16_t* o = static_cast<uint16_t*>(a.out) + at * D + d;
 #pragma unroll
-        for (int e = 0; e < D / 16; ++e) part.out[at * D + d + e] = y[e] * scale;
-        if (d == 0) part.log[at] = log;
-      } else {
-        const int64_t at = (s.first + i) * a.Hq + hq;
-        uint16_t* o = static_cast<uint16_t*>(a.out) + at * D + d;
-#pragma unroll
-        for (int e = 0; e < D / 16; ++e)
-          o[e] = __builtin_bit_cast(uint16_t, to_out<T>(y[e] * scale));
-        if (a.lse && d == 0) a.lse[at] = log * kLn2;
-      }
+      for (int e = 0; e < D / 16; ++e) o[e] = __builtin_bit_cast(uint16_t, to_out<T>(y[e] * scale));
+      if (a.lse && d == 0) a.lse[at] = log * kLn2;
     }
   }
 }
 
-// Grid: (max_q Hq, B): a row's parts weighted by their sums.  The four waves of a workgroup
-// take every fourth part, eight at a time so that their loads are in flight together.
+// Up to sixteen rows a key/value head, the waves of a workgroup on every NW-th step; two
+// waves share a SIMD.
+template <int D, typename T, int NW, bool WHOLE>
+__global__ __launch_bounds__(64 * NW, 2) void kv_attend_split_kernel(
+    KvAttend a, Shares shares, Plan plan) {
+  __shared__ alignas(16) Joint<D, NW> joint;
+  if constexpr (WHOLE) {
+    const int b = blockIdx.z, h = blockIdx.y;
+    const Sequence s = sequence_of(a, b);
+    if (s.n <= 0) return;
+    const Steps steps = steps_of(a, s);
+    attend_steps<D, T, NW>(a, shares, joint, s, b, h, steps.first, steps.first + steps.count, -1);
+    return;
+  }
+  // Where in the batch's steps this workgroup's share begins: the steps of all sequences,
+  // summed by the threads, a run of sequences each.
+  __shared__ int64_t wave_sums[NW];
+  __shared__ int64_t found_start;
+  __shared__ int found;
+  const int h = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int run = (a.B + 64 * NW - 1) / (64 * NW), b0 = min(t * run, a.B), b1 = min(b0 + run, a.B);
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) mine += steps_of(a, sequence_of(a, b)).count;
+  int64_t before = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t x = __shfl_up(before, d);
+    before += lane >= d ? x : 0;
+  }
+  if (lane == 63) wave_sums[wave] = before;
+  before -= mine;
+  __syncthreads();
+  int64_t all = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    before += w < wave ? wave_sums[w] : 0;
+    all += wave_sums[w];
+  }
+  const int64_t share = max((all + gridDim.x - 1) / (int64_t)gridDim.x, (int64_t)plan.least);
+  const int64_t from = blockIdx.x * share, to = min(from + share, all);
+  if (from >= all) return;
+  if (before <= from && from < before + mine) {
+    int b = b0;
+    for (;; ++b) {
+      const int n = steps_of(a, sequence_of(a, b)).count;
+      if (from < before + n) break;
+      before += n;
+    }
+    found = b;
+    found_start = before;
+  }
+  __syncthreads();
+  int b = __builtin_amdgcn_readfirstlane(found);
+  int64_t start = found_start;
+  for (int64_t at = from; at < to; ++b) {
+    const Sequence s = sequence_of(a, b);
+    const Steps steps = steps_of(a, s);
+    if (steps.count == 0) continue;
+    const int64_t end = start + steps.count;
+    const int64_t part0 = start / share, used = (end - 1) / share - part0 + 1;
+    if (h == 0 && at == start && t == 0) shares.where[b] = {(int)part0 + b, (int)used};
+    const int s0 = __builtin_amdgcn_readfirstlane((int)(at - start));
+    const int s1 = __builtin_amdgcn_readfirstlane((int)(min(to, end) - start));
+    attend_steps<D, T, NW>(a, shares, joint, s, b, h, steps.first + s0, steps.first + s1,
+                               used > 1 ? (int64_t)blockIdx.x + b : -1);
+    at = start = end;
+    __syncthreads();
+  }
+}
+
+// A row's parts, weighted by their sums.  Grid: (max_q Hq, B) rows, one a wave, or (`per` = 4)
+// a workgroup, whose waves take every fourth part; eight at a time, so that their loads are
+// in flight together.
 template <int D, typename T>
-__global__ __launch_bounds__(64 * kWaves) void kv_attend_join_kernel(
-    KvAttend a, Part part, Plan plan, int per) {
+__global__ __launch_bounds__(64 * kWaves) void kv_attend_join_kernel(KvAttend a, Shares shares,
+                                                                     Plan plan, int per) {
   __shared__ float out[kWaves][D], sums[kWaves];
-  const int lane = threadIdx.x & 63;
-  // This wave's share of its row: every `per`-th part.
+  const int lane = threadIdx.x & 63, b = blockIdx.y;
   int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int b = blockIdx.y;
   const int row = blockIdx.x * (kWaves / per) + wave / per, i = row / a.Hq, hq = row - i * a.Hq;
   wave %= per;
   const Sequence s = sequence_of(a, b);
-  const int G = a.Hq / a.cache.H, chunks = plan.chunks;
+  const int H = a.cache.H, G = a.Hq / H, h = hq / G;
   int used = 0;
-  if (i < s.n) used = parts_of(a, s, plan, G, (i * G + hq % G) / plan.rows * plan.rows).used;
+  int64_t at = 0, stride = 1;
+  if (i < s.n && plan.form == kShares) {
+    const int slot = uniform_load(&shares.where[b].slot);
+    used = uniform_load(&shares.where[b].used);
+    stride = H * (int64_t)a.max_q * G;
+    at = slot * stride + h * ((int64_t)a.max_q * G) + i * G + hq - h * G;
+  } else if (i < s.n) {
+    // As kv_attend_prompt_kernel.
+    const int r0 = (i * G + hq - h * G) / plan.rows * plan.rows;
+    const int r1 = min(r0 + plan.rows, s.n * G) - 1;
+    const int first = row_begin(a, s, r0 / G) / plan.step;
+    const int last = (row_end(s, r1 / G) + plan.step - 1) / plan.step;
+    const int each = max((last - first + plan.chunks - 1) / plan.chunks, plan.least);
+    used = (last - first + each - 1) / each;
+    at = (((int64_t)b * a.max_q + i) * a.Hq + hq) * plan.chunks;
+  }
   const bool in = used > 1;  // a row of one part is done
   if (per == kWaves && !in) return;
-  const int64_t at = (((int64_t)b * a.max_q + i) * a.Hq + hq) * chunks;
+  const Part& part = shares.part;
   float top = -INFINITY;
-  for (int c = lane; c < used; c += 64) top = fmaxf(top, part.log[at + c]);
+  for (int c = lane; in && c < used; c += 64) top = fmaxf(top, part.log[at + c * stride]);
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
   const float base = top == -INFINITY ? 0.0f : top;
@@ -458,7 +482,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attend_join_kernel(
     float log[kMany], x[kMany][kE];
 #pragma unroll
     for (int m = 0; m < kMany; ++m) {
-      const int64_t from = at + min(c + m * per, used - 1);
+      const int64_t from = at + min(c + m * per, used - 1) * stride;
       log[m] = part.log[from];
 #pragma unroll
       for (int e = 0; e < kE; ++e) x[m][e] = part.out[from * D + lane * kE + e];
@@ -499,60 +523,71 @@ Plan plan_of(int B, int Hq, int H, int max_q, int64_t max_length, int64_t window
   const int64_t length =
       std::min<int64_t>(window ? std::min(max_length, window + max_q - 1) : max_length, kKvMaxLength);
   Plan p = {};
-  int64_t groups = 1, slots;
-  if (rows > 64) {
-    // 256 rows a workgroup, one of which a CU holds, or 128 (two).
-    p.prompt = true;
+  p.chunks = 1;
+  if (rows > 16) {
+    // 256 rows a workgroup, one of which a CU holds, or 128 (two); few of them: their
+    // tokens in parts.
+    p.form = kPrompt;
     p.rows = rows > 128 ? 256 : 128;
+    p.waves = p.rows / 32;
     p.step = p.rows / 2;
-    p.least = 2;
-    groups = (rows + p.rows - 1) / p.rows;
-    slots = cus * (256 / p.rows);
-  } else {
-    // As many workgroups as the device holds at once: each has the same tokens to read, so
-    // a second round would only add its start and end (131072 tokens of 8 heads: 36 us in
-    // one round, 41 in two, 49 in four).
-    p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
-    p.step = kStep;
-    p.least = kWaves;
-    slots = cus * (p.rows == 16 ? 3 : 1);
+    const int64_t steps = (length + p.step - 1) / p.step + 1;
+    const int64_t wgs = (rows + p.rows - 1) / p.rows * B * H, slots = cus * (256 / p.rows);
+    p.chunks = (int)std::max<int64_t>(1, std::min((steps + 1) / 2, slots / wgs));
+    p.least = (int)std::max<int64_t>(2, (steps + p.chunks - 1) / p.chunks);
+    return p;
   }
-  const int64_t steps = (length + p.step - 1) / p.step + 1, wgs = groups * B * H;
-  const int64_t want = p.prompt ? slots / wgs : (slots + wgs - 1) / wgs;
-  p.chunks = (int)std::max<int64_t>(1, std::min((steps + p.least - 1) / p.least, want));
-  p.least = (int)std::max<int64_t>(p.least, (steps + p.chunks - 1) / p.chunks);
+  p.step = kStep;
+  // Up to 1024 tokens by the eight waves of one workgroup: four steps a wave cost less than
+  // the second kernel (8 sequences of 1000 tokens, 64/8 heads: 11.5 us, 14.0 split).
+  p.form = length <= 1024 ? kWhole : kShares;
+  p.waves = p.form == kWhole ? 8 : kWaves;
+  // As many workgroups as the device holds at once: a second round would only add its start
+  // and end (131072 tokens of 8 heads: 36 us in one round, 41 in two, 49 in four).
+  p.wgs = (int)std::max<int64_t>(1, 2 * cus / H);
+  p.least = kWaves;
   return p;
+}
+
+// Bytes of the parts, before what says where they are.
+int64_t part_bytes(const Plan& p, int D, int B, int Hq, int max_q) {
+  const int64_t rows = (int64_t)max_q * Hq;
+  if (p.form == kShares) return (p.wgs + B) * rows * (D + 1) * 4;
+  return p.chunks > 1 ? B * rows * p.chunks * (D + 1) * 4 : 0;
 }
 
 template <int D, typename T>
 int attend(const KvAttend& a, void* ws, hipStream_t stream) {
   const Plan p = plan_of(a.B, a.Hq, a.cache.H, a.max_q, a.max_length, a.window);
-  Part part = {nullptr, nullptr};
-  if (p.chunks > 1) {
-    part.out = static_cast<float*>(ws);
-    part.log = part.out + (int64_t)a.B * a.max_q * a.Hq * p.chunks * D;
+  const bool joins = p.form == kShares || p.chunks > 1;
+  Shares shares = {};
+  if (joins) {
+    const int64_t bytes = part_bytes(p, D, a.B, a.Hq, a.max_q);
+    shares.part.out = static_cast<float*>(ws);
+    shares.part.log = shares.part.out + bytes / 4 / (D + 1) * D;
+    shares.where = reinterpret_cast<Where*>(static_cast<uint8_t*>(ws) + (bytes + 15) / 16 * 16);
   }
   // Timing events, if armed, span both kernels.
   const KernelEvents ev = take_kernel_events();
-  arm_kernel_events({ev.start, p.chunks > 1 ? nullptr : ev.stop});
-  const dim3 grid(p.chunks, a.cache.H, a.B), block(64 * kWaves);
+  arm_kernel_events({ev.start, joins ? nullptr : ev.stop});
+  const dim3 grid = p.form == kShares ? dim3(p.wgs, a.cache.H, 1) : dim3(1, a.cache.H, a.B);
+  const dim3 block(64 * p.waves);
   int rc = 0;
-  if (p.prompt)
-    rc = kv_attend_prompt(a, D, std::is_same<T, bf16>::value, part, p.rows / 32, p.chunks, p.least,
-                          stream);
-  else if (p.rows == 16)
-    launch(kv_attend_split_kernel<D, T, 1>, grid, block, stream, a, part, p);
-  else if (p.rows == 32)
-    launch(kv_attend_split_kernel<D, T, 2>, grid, block, stream, a, part, p);
+  if (p.form == kPrompt)
+    rc = kv_attend_prompt(a, D, std::is_same<T, bf16>::value, shares.part, p.waves, p.chunks,
+                          p.least, stream);
+  else if (p.form == kWhole)
+    launch(kv_attend_split_kernel<D, T, 8, true>, grid, block, stream, a, shares, p);
   else
-    launch(kv_attend_split_kernel<D, T, 4>, grid, block, stream, a, part, p);
+    launch(kv_attend_split_kernel<D, T, kWaves, false>, grid, block, stream, a, shares, p);
   if (rc) return rc;
-  if (p.chunks > 1) {
-    // A row's parts by one wave, or, where there are many, by four.
-    const int per = p.chunks <= 16 ? 1 : kWaves, rows = kWaves / per;
+  if (joins) {
+    // One wave a row where there are rows enough, else four.
+    const int per = (int64_t)a.max_q * a.Hq * a.B >= 4 * cu_count() ? 1 : kWaves;
+    const int rows = kWaves / per;
     arm_kernel_events({nullptr, ev.stop});
-    launch(kv_attend_join_kernel<D, T>, dim3((a.max_q * a.Hq + rows - 1) / rows, a.B), block, stream,
-           a, part, p, per);
+    launch(kv_attend_join_kernel<D, T>, dim3((a.max_q * a.Hq + rows - 1) / rows, a.B),
+           dim3(64 * kWaves), stream, a, shares, p, per);
   }
   return launch_status("kv_attention");
 }
@@ -562,7 +597,8 @@ int attend(const KvAttend& a, void* ws, hipStream_t stream) {
 int64_t kv_attention_workspace_bytes(int D, int B, int Hq, int H, int max_q, int64_t max_length,
                                      int64_t window) {
   const Plan p = plan_of(B, Hq, H, max_q, max_length, window);
-  return p.chunks > 1 ? (int64_t)B * max_q * Hq * p.chunks * (D + 1) * 4 : 0;
+  const int64_t bytes = part_bytes(p, D, B, Hq, max_q);
+  return p.form == kShares ? (bytes + 15) / 16 * 16 + B * (int64_t)sizeof(Where) : bytes;
 }
 
 int kv_attention(const KvAttend& a, int D, bool is_bf16, void* ws, hipStream_t stream) {
