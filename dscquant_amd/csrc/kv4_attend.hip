@@ -39,7 +39,6 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kStep = 2 * kKvTile;  // tokens of a step
-constexpr int kAhead = 2;           // steps whose codes are on their way
 
 // What a lane reads of a 16-token tile.
 template <int D>
@@ -227,30 +226,24 @@ struct Rows {
   }
 
   // The steps first, first + stride, ... below `last` (tokens / 32).  While one step is
-  // computed the next two steps' codes are on their way, and the one's after them pages.
+  // computed the next one's codes are on their way, and the one's after it pages.  The body
+  // stands once and the codes move from register to register: a second copy of it would cost
+  // a short run more, in instructions fetched for the first time, than the moves do.
   __device__ __forceinline__ void run(const Pages<D>& g, int first, int last, int stride, int lane) {
     if (first >= last) return;
+    Tile<D> a = load_tile<D>(g, place_of(g.places, 2 * first));
+    Tile<D> b = load_tile<D>(g, place_of(g.places, 2 * first + 1));
+    Place pa = place_of(g.places, 2 * (first + stride));
+    Place pb = place_of(g.places, 2 * (first + stride) + 1);
     const Masks masks;
-    Tile<D> a[kAhead + 1], b[kAhead + 1];
-    Place pa = place_of(g.places, 2 * first), pb = place_of(g.places, 2 * first + 1);
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      a[i] = load_tile<D>(g, pa);
-      b[i] = load_tile<D>(g, pb);
-      pa = place_of(g.places, 2 * (first + (i + 1) * stride));
-      pb = place_of(g.places, 2 * (first + (i + 1) * stride) + 1);
-    }
-    for (int st = first;; st += (kAhead + 1) * stride) {
-#pragma unroll
-      for (int i = 0; i <= kAhead; ++i) {
-        const int at = st + i * stride, to = (i + kAhead) % (kAhead + 1);
-        a[to] = load_tile<D>(g, pa);
-        b[to] = load_tile<D>(g, pb);
-        pa = place_of(g.places, 2 * (at + (kAhead + 1) * stride));
-        pb = place_of(g.places, 2 * (at + (kAhead + 1) * stride) + 1);
-        step(a[i], b[i], at * kStep, lane, masks);
-        if (at + stride >= last) return;
-      }
+#pragma unroll 1
+    for (int at = first; at < last; at += stride) {
+      const Tile<D> na = load_tile<D>(g, pa), nb = load_tile<D>(g, pb);
+      pa = place_of(g.places, 2 * (at + 2 * stride));
+      pb = place_of(g.places, 2 * (at + 2 * stride) + 1);
+      step(a, b, at * kStep, lane, masks);
+      a = na;
+      b = nb;
     }
   }
 };
