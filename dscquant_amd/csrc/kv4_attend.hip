@@ -250,12 +250,13 @@ struct Rows {
 
 // The launch's plan.
 //   kWhole   a workgroup takes all tokens of its rows: grid (1, H, B), one kernel;
+//   kParts   a sequence's tokens in up to `chunks` parts of at least `least` steps (step
+//            tokens each): grid (chunks, H, B); a second kernel joins the parts;
 //   kShares  each of `wgs` workgroups a head takes the same share of the batch's steps
-//            (step tokens of one sequence each, in order, at least `least`), whichever
-//            sequences that is; a second kernel joins the parts of a sequence;
-//   kPrompt  kv4_prompt.hip: groups of `rows` rows, their tokens in up to `chunks` parts of
-//            at least `least` steps, joined likewise where chunks > 1.
-enum Form { kWhole, kShares, kPrompt };
+//            (in order, at least `least`), whichever sequences that is, joined likewise;
+//   kPrompt  kv4_prompt.hip: groups of `rows` rows, their tokens in parts as in kParts,
+//            joined where chunks > 1.
+enum Form { kWhole, kParts, kShares, kPrompt };
 struct Plan {
   Form form;
   int rows, waves, step, wgs, chunks, least;
@@ -305,11 +306,12 @@ struct Joint {  // LDS in which the waves of a workgroup join their results
 };
 
 // Steps from .. to - 1 of sequence b for head h, joined over the waves: the rows' result, or
-// (slot >= 0) their part.
+// (slot >= 0) their part, the slot-th of `chunks` of each row or in a slot of its own.
 template <int D, typename T, int NW>
 __device__ __forceinline__ void attend_steps(const KvAttend& a, const Shares& shares,
                                              Joint<D, NW>& joint, const Sequence& s, int b,
-                                             int h, int from, int to, int64_t slot) {
+                                             int h, int from, int to, int64_t slot,
+                                             int chunks = 0) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int G = a.Hq / a.cache.H, count = s.n * G;
   Rows<D> rows;
@@ -346,7 +348,9 @@ __device__ __forceinline__ void attend_steps(const KvAttend& a, const Shares& sh
     const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
     const float log = sum == 0.0f ? -INFINITY : base + __builtin_amdgcn_logf(sum);
     if (slot >= 0) {
-      const int64_t at = (slot * a.cache.H + h) * ((int64_t)a.max_q * G) + row;
+      const int i = row / G, hq = h * G + row - i * G;
+      const int64_t at = chunks ? (((int64_t)b * a.max_q + i) * a.Hq + hq) * chunks + slot
+                                : (slot * a.cache.H + h) * ((int64_t)a.max_q * G) + row;
 #pragma unroll
       for (int e = 0; e < D / 16; ++e) shares.part.out[at * D + d + e] = y[e] * scale;
       if (d == 0) shares.part.log[at] = log;
@@ -363,16 +367,26 @@ __device__ __forceinline__ void attend_steps(const KvAttend& a, const Shares& sh
 
 // Up to sixteen rows a key/value head, the waves of a workgroup on every NW-th step; two
 // waves share a SIMD.
-template <int D, typename T, int NW, bool WHOLE>
+template <int D, typename T, int NW, Form FORM>
 __global__ __launch_bounds__(64 * NW, 2) void kv_attend_split_kernel(
     KvAttend a, Shares shares, Plan plan) {
   __shared__ alignas(16) Joint<D, NW> joint;
-  if constexpr (WHOLE) {
+  if constexpr (FORM != kShares) {
     const int b = blockIdx.z, h = blockIdx.y;
     const Sequence s = sequence_of(a, b);
     if (s.n <= 0) return;
     const Steps steps = steps_of(a, s);
-    attend_steps<D, T, NW>(a, shares, joint, s, b, h, steps.first, steps.first + steps.count, -1);
+    int from = steps.first, to = from + steps.count;
+    int64_t slot = -1;
+    if constexpr (FORM == kParts) {
+      const int each = max((steps.count + plan.chunks - 1) / plan.chunks, plan.least);
+      from += blockIdx.x * each;
+      if (from >= to) return;
+      slot = steps.count > each ? (int64_t)blockIdx.x : -1;
+      to = min(from + each, to);
+    }
+    attend_steps<D, T, NW>(a, shares, joint, s, b, h, from, to, slot,
+                           FORM == kParts ? plan.chunks : 0);
     return;
   }
   // Where in the batch's steps this workgroup's share begins: the steps of all sequences,
@@ -452,13 +466,13 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attend_join_kernel(KvAttend a,
     stride = H * (int64_t)a.max_q * G;
     at = slot * stride + h * ((int64_t)a.max_q * G) + i * G + hq - h * G;
   } else if (i < s.n) {
-    // As kv_attend_prompt_kernel.
+    // As the kernels of parts.
     const int r0 = (i * G + hq - h * G) / plan.rows * plan.rows;
     const int r1 = min(r0 + plan.rows, s.n * G) - 1;
     const int first = row_begin(a, s, r0 / G) / plan.step;
     const int last = (row_end(s, r1 / G) + plan.step - 1) / plan.step;
     const int each = max((last - first + plan.chunks - 1) / plan.chunks, plan.least);
-    used = (last - first + each - 1) / each;
+    used = (max(last - first, 1) + each - 1) / each;
     at = (((int64_t)b * a.max_q + i) * a.Hq + hq) * plan.chunks;
   }
   const bool in = used > 1;  // a row of one part is done
@@ -530,15 +544,28 @@ Plan plan_of(int B, int Hq, int H, int max_q, int64_t max_length, int64_t window
     p.least = (int)std::max<int64_t>(2, (steps + p.chunks - 1) / p.chunks);
     return p;
   }
+  p.rows = 16;
   p.step = kStep;
   // Up to 1024 tokens by the eight waves of one workgroup: four steps a wave cost less than
   // the second kernel (8 sequences of 1000 tokens, 64/8 heads: 11.5 us, 14.0 split).
-  p.form = length <= 1024 ? kWhole : kShares;
+  p.form = length <= 1024 ? kWhole : kParts;
   p.waves = p.form == kWhole ? 8 : kWaves;
+  if (p.form == kWhole) return p;
   // As many workgroups as the device holds at once: a second round would only add its start
-  // and end (131072 tokens of 8 heads: 36 us in one round, 41 in two, 49 in four).
+  // and end (131072 tokens of 8 heads: 36 us in one round, 41 in two, 49 in four).  With
+  // four of them a sequence or more, parts are a sequence's own; with fewer, a ragged batch
+  // would leave most of the device waiting for its longest (64 sequences of 1 to 4096
+  // tokens: 57 us in two parts each, 46 in equal shares), but a share that spans two
+  // sequences begins and ends twice (8 sequences of 2000: 20 us, 17 in parts).
   p.wgs = (int)std::max<int64_t>(1, 2 * cus / H);
   p.least = kWaves;
+  if (B > p.wgs / 4) {
+    p.form = kShares;
+  } else {
+    const int64_t steps = (length + kStep - 1) / kStep + 1;
+    p.chunks = (int)std::min<int64_t>(p.wgs / B, (steps + p.least - 1) / p.least);
+    p.least = (int)std::max<int64_t>(p.least, (steps + p.chunks - 1) / p.chunks);
+  }
   return p;
 }
 
@@ -563,16 +590,18 @@ int attend(const KvAttend& a, void* ws, hipStream_t stream) {
   // Timing events, if armed, span both kernels.
   const KernelEvents ev = take_kernel_events();
   arm_kernel_events({ev.start, joins ? nullptr : ev.stop});
-  const dim3 grid = p.form == kShares ? dim3(p.wgs, a.cache.H, 1) : dim3(1, a.cache.H, a.B);
+  const dim3 grid = p.form == kShares ? dim3(p.wgs, a.cache.H, 1) : dim3(p.chunks, a.cache.H, a.B);
   const dim3 block(64 * p.waves);
   int rc = 0;
   if (p.form == kPrompt)
     rc = kv_attend_prompt(a, D, std::is_same<T, bf16>::value, shares.part, p.waves, p.chunks,
                           p.least, stream);
   else if (p.form == kWhole)
-    launch(kv_attend_split_kernel<D, T, 8, true>, grid, block, stream, a, shares, p);
+    launch(kv_attend_split_kernel<D, T, 8, kWhole>, grid, block, stream, a, shares, p);
+  else if (p.form == kParts)
+    launch(kv_attend_split_kernel<D, T, kWaves, kParts>, grid, block, stream, a, shares, p);
   else
-    launch(kv_attend_split_kernel<D, T, kWaves, false>, grid, block, stream, a, shares, p);
+    launch(kv_attend_split_kernel<D, T, kWaves, kShares>, grid, block, stream, a, shares, p);
   if (rc) return rc;
   if (joins) {
     // One wave a row where there are rows enough, else four.
