@@ -58,27 +58,39 @@ def _check_cache(cache: torch.Tensor):
     return pages, heads, page_size, row - 8
 
 
-def _check_rows(name: str, x: torch.Tensor, cache: torch.Tensor, tokens: int, heads, dim: int):
-    if x.device != cache.device:
+# The checks read each property of a tensor once (a call's host time is its checks, its
+# allocations and the call through ctypes) and look for what is wrong only if something is.
+
+def _rows(name: str, x: torch.Tensor, index: int, shape) -> tuple:
+    """The strides of rows [tokens, heads, head_dim] on device ``index``."""
+    if x.shape == shape and x.dtype in _DTYPES and x.get_device() == index:
+        strides = x.stride()
+        if strides[2] == 1 or not x.numel():
+            if x.requires_grad and torch.is_grad_enabled():
+                raise RuntimeError(_NO_GRAD)
+            return strides
+    if x.get_device() != index:
         raise RuntimeError("All buffers must be on the same device")
     if x.dtype not in _DTYPES:
         raise RuntimeError("Only FP16 and BF16 inputs are supported")
-    if x.dim() != 3 or x.size(0) != tokens or x.size(2) != dim or (
-            heads is not None and x.size(1) != heads):
-        raise RuntimeError(f"kv4: {name} must be [{tokens}, {'heads' if heads is None else heads}, "
-                           f"{dim}] (got {list(x.shape)})")
-    if x.stride(2) != 1 and x.numel():
-        raise RuntimeError(f"kv4: the elements of a head of {name} must be contiguous")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError(_NO_GRAD)
+    if x.shape != shape:
+        raise RuntimeError(f"kv4: {name} must be {list(shape)} (got {list(x.shape)})")
+    raise RuntimeError(f"kv4: the elements of a head of {name} must be contiguous")
 
 
-def _check_index(name: str, t: torch.Tensor, cache: torch.Tensor, dtype, shape) -> None:
-    if t.device != cache.device:
+def _heads(name: str, x: torch.Tensor, dim: int) -> int:
+    if x.dim() != 3:
+        raise RuntimeError(f"kv4: {name} must be [tokens, heads, {dim}] (got {list(x.shape)})")
+    return x.size(1)
+
+
+def _check_index(name: str, t: torch.Tensor, index: int, dtype, shape) -> None:
+    if t.dtype is dtype and t.shape == shape and t.get_device() == index and t.is_contiguous():
+        return
+    if t.get_device() != index:
         raise RuntimeError("All buffers must be on the same device")
-    if t.dtype != dtype or not t.is_contiguous() or tuple(t.shape) != tuple(shape):
-        raise RuntimeError(f"kv4: {name} must be contiguous {str(dtype)[6:]} {list(shape)} "
-                           f"(got {str(t.dtype)[6:]} {list(t.shape)})")
+    raise RuntimeError(f"kv4: {name} must be contiguous {str(dtype)[6:]} {list(shape)} "
+                       f"(got {str(t.dtype)[6:]} {list(t.shape)})")
 
 
 def slots(tables: torch.Tensor, sequences: torch.Tensor, places: torch.Tensor,
@@ -102,39 +114,43 @@ def append(cache: torch.Tensor, q, k: torch.Tensor, v: torch.Tensor, slots: torc
     NaN queries, nothing stored.  ``rotate`` stores H_D k and returns H_D q / D (the same
     scores; the activations' Hadamard for keys with a few large channels)."""
     pages, H, P, D = _check_cache(cache)
+    dev = cache.get_device()
     T = k.size(0)
-    _check_rows("k", k, cache, T, H, D)
-    _check_rows("v", v, cache, T, H, D)
-    if v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
+    k_strides = _rows("k", k, dev, (T, H, D))
+    v_strides = _rows("v", v, dev, (T, H, D))
+    if v.dtype is not k.dtype or (q is not None and q.dtype is not k.dtype):
         raise RuntimeError("kv4: q, k and v must have the same dtype")
-    Hq = 0
+    Hq, q_args, out = 0, (None, 0, 0), None
     if q is not None:
-        _check_rows("q", q, cache, T, None, D)
-        Hq = q.size(1)
-    _check_index("slots", slots, cache, torch.int64, (T,))
-    rows = R = 0
+        Hq = _heads("q", q, D)
+        q_strides = _rows("q", q, dev, (T, Hq, D))
+        if Hq == 0 or Hq > 4096:
+            raise RuntimeError(f"kv4: 1 to 4096 query heads (got {Hq})")
+        q_args = (q.data_ptr(), q_strides[0], q_strides[1])
+    _check_index("slots", slots, dev, torch.int64, (T,))
+    turn = (None, None, None, 0, 0)
     if cos is not None or sin is not None or positions is not None:
         if cos is None or sin is None or positions is None:
             raise RuntimeError("kv4: cos, sin and positions go together")
-        rows, R = (cos.size(0), 2 * cos.size(1)) if cos.dim() == 2 else (0, 0)
-        if rows == 0 or R % 16 or not 16 <= R <= D:
+        rows, half = cos.shape if cos.dim() == 2 else (0, 0)
+        if rows == 0 or half % 8 or not 8 <= half <= D // 2:
             raise RuntimeError("kv4: cos and sin must be [rows, R / 2] with R a multiple of 16 "
                                f"up to {D} (got {list(cos.shape)})")
-        _check_index("cos", cos, cache, torch.float32, (rows, R // 2))
-        _check_index("sin", sin, cache, torch.float32, (rows, R // 2))
-        _check_index("positions", positions, cache, torch.int64, (T,))
-    dev = cache.device
-    _lib.require_gfx950(dev)
-    out = None if q is None else torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
+        _check_index("cos", cos, dev, torch.float32, (rows, half))
+        _check_index("sin", sin, dev, torch.float32, (rows, half))
+        _check_index("positions", positions, dev, torch.int64, (T,))
+        turn = (positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), rows, 2 * half)
+    device = cache.device
+    _lib.require_gfx950(device)
+    if q is not None:
+        out = q.new_empty((T, Hq, D))
     if T == 0:
         return out
-    with _lib.on(dev):
-        _lib.call("dscq_kv_append", *((None, 0, 0) if not Hq else
-                                      (q.data_ptr(), q.stride(0), q.stride(1))),
-                  k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-                  _DTYPES[k.dtype], T, Hq, H, D, _lib.ptr(positions), _lib.ptr(cos), _lib.ptr(sin),
-                  rows, R, 1 if interleaved else 0, 1 if rotate else 0, slots.data_ptr(),
-                  cache.data_ptr(), pages, P, _lib.ptr(out), _lib.stream(dev))
+    with _lib.on(device):
+        _lib.call("dscq_kv_append", *q_args, k.data_ptr(), k_strides[0], k_strides[1], v.data_ptr(),
+                  v_strides[0], v_strides[1], _DTYPES[k.dtype], T, Hq, H, D, *turn,
+                  1 if interleaved else 0, 1 if rotate else 0, slots.data_ptr(), cache.data_ptr(),
+                  pages, P, None if out is None else out.data_ptr(), _lib.stream(device))
     return out
 
 
@@ -145,10 +161,11 @@ def read(cache: torch.Tensor, slots: torch.Tensor, dtype=torch.float16, rotate: 
     pages, H, P, D = _check_cache(cache)
     if dtype not in _DTYPES:
         raise RuntimeError("Only FP16 and BF16 inputs are supported")
-    _check_index("slots", slots, cache, torch.int64, (slots.numel(),))
     T, dev = slots.numel(), cache.device
+    _check_index("slots", slots, cache.get_device(), torch.int64, (T,))
     _lib.require_gfx950(dev)
-    k, v = (torch.empty((T, H, D), dtype=dtype, device=dev) for _ in range(2))
+    k = torch.empty((T, H, D), dtype=dtype, device=dev)
+    v = k.new_empty((T, H, D))
     if T:
         with _lib.on(dev):
             _lib.call("dscq_kv_read", cache.data_ptr(), pages, P, H, D, slots.data_ptr(), T,
@@ -173,19 +190,19 @@ def attention(cache: torch.Tensor, q: torch.Tensor, tables: torch.Tensor, length
     query's softmax sum, fp32 [T, Hq] (-inf for one that sees none), with which results over
     parts of a context are joined."""
     pages, H, P, D = _check_cache(cache)
-    T = q.size(0)
-    _check_rows("q", q, cache, T, None, D)
-    Hq = q.size(1)
+    index = cache.get_device()
+    T, Hq = q.size(0), _heads("q", q, D)
+    strides = _rows("q", q, index, (T, Hq, D))
     if Hq == 0 or Hq % H or Hq > 4096:
         raise RuntimeError("kv4: query heads must be a multiple of the cache's heads, up to 4096")
     if tables.dim() != 2 or tables.size(0) > 65535:
         raise RuntimeError("kv4: tables must be [B, width] with B up to 65535")
     B, width = tables.shape
-    _check_index("tables", tables, cache, torch.int32, (B, width))
-    _check_index("lengths", lengths, cache, torch.int32, (B,))
+    _check_index("tables", tables, index, torch.int32, (B, width))
+    _check_index("lengths", lengths, index, torch.int32, (B,))
     max_q, window = int(max_q), int(window)
     if starts is not None:
-        _check_index("starts", starts, cache, torch.int32, (B + 1,))
+        _check_index("starts", starts, index, torch.int32, (B + 1,))
     elif max_q != 1 or T != B:
         raise RuntimeError("kv4: without starts every sequence has one query")
     max_length = width * P if max_length is None else int(max_length)
@@ -196,16 +213,17 @@ def attention(cache: torch.Tensor, q: torch.Tensor, tables: torch.Tensor, length
         raise RuntimeError(f"kv4: scale must be positive (got {scale})")
     dev = cache.device
     _lib.require_gfx950(dev)
-    out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
-    lse = torch.empty((T, Hq), dtype=torch.float32, device=dev) if return_lse else None
+    out = q.new_empty((T, Hq, D))
+    lse = q.new_empty((T, Hq), dtype=torch.float32) if return_lse else None
     if T and B and max_q:
         with _lib.on(dev):
+            # The plan, and with it the scratch, depends on the device's compute units.
             need = int(_lib.lib().dscq_kv_attention_workspace_bytes(B, Hq, H, D, max_q, max_length,
                                                                     window))
             ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need > 0 else None
-            _lib.call("dscq_kv_attention", q.data_ptr(), q.stride(0), q.stride(1),
-                      _DTYPES[q.dtype], T, Hq, cache.data_ptr(), pages, P, H, D, _lib.ptr(tables),
-                      width, lengths.data_ptr(), _lib.ptr(starts), B, max_q, max_length, scale,
-                      window, out.data_ptr(), _lib.ptr(lse), _lib.ptr(ws), max(need, 0),
+            _lib.call("dscq_kv_attention", q.data_ptr(), strides[0], strides[1], _DTYPES[q.dtype],
+                      T, Hq, cache.data_ptr(), pages, P, H, D, _lib.ptr(tables), width,
+                      lengths.data_ptr(), None if starts is None else starts.data_ptr(), B, max_q,
+                      max_length, scale, window, out.data_ptr(), _lib.ptr(lse), _lib.ptr(ws), max(need, 0),
                       _lib.stream(dev))
     return (out, lse) if return_lse else out
