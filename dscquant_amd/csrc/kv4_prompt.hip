@@ -1,14 +1,30 @@
 // Attention of many rows over the 4-bit key/value cache: prompts and their chunks.
 //
 // The mathematics of kv4_attend.hip.  With hundreds of rows a key/value head the products
-// bound the time, and next to them the softmax (an exponential, six other operations a
-// score) and the unpacking, so the codes are unpacked once for a workgroup: its waves take
-// 64 tokens in turn, a 16-token tile each, and leave keys and values as fp16 in LDS (twice,
-// so that the next tokens are written while these are used); every wave multiplies all of
-// them with rows of its own, 32 or 64 that it holds in registers.  32 x 32 x 16 products:
-// S^T (32 tokens x 32 rows) leaves lane (c, h) = (lane % 32, lane / 32) the scores of row c
-// and tokens 8 a + 4 h + i, which as they lie are the operand of O^T += V^T P^T over the
-// token order 16 s + 4 h + 0..3, 16 s + 8 + 4 h + 0..3; V^T is stored in that order.
+// bound the time, and next to them the softmax (an exponential and four other operations a
+// score) and the unpacking, so the codes are unpacked once for a workgroup: its four or
+// eight waves take 64 or 128 tokens in turn, a 16-token tile each, and leave keys and values
+// as fp16 in LDS (twice, so that the next tokens are written while these are used); every
+// wave multiplies all of them with 32 rows of its own, which it holds in registers.
+// 32 x 32 x 16 products: S^T (32 tokens x 32 rows) leaves lane (c, h) = (lane % 32, lane / 32)
+// the scores of row c and tokens 8 a + 4 h + i, which as they lie are the operand of
+// O^T += V^T P^T over the token order 16 s + 4 h + 0..3, 16 s + 8 + 4 h + 0..3; V^T is stored
+// in that order.
+//
+// A value's scale f' goes into the exponent: with t = s log2 e + log2 f' the weight times the
+// scale is 2^(t - reference) at once, and the softmax sum adds it times 1 / f'.  The products
+// start from (log2 f') / (f scale log2 e), so one multiply-add makes t of them.  The reference
+// follows the row's largest t, which may pass it by eight binary places before it moves.
+//
+// Measured: 4096 queries after 12288 tokens, 64 query and 8 key/value heads of 128, bf16:
+// 1.96 ms (980 TFLOP/s of 4 D operations a visible pair; a large library product of the
+// type reaches 1190).  The matrix pipes are busy 44% of the cycles, a third of that beside
+// vector instructions (2.0 GHz under this load).  Without its exponentials the kernel would
+// take 3% less, without reading values from LDS 2%, without unpacking 4%, with an eighth of
+// either product 20%.  2048 queries of 32 heads, fp16: 70 us (490 TFLOP/s): 256 workgroups,
+// the longest of them 64 steps of 1.2 us one after another.  64 rows a wave (half the LDS
+// reads a product) do not fit its registers: 6.1 ms.  Instructions interleaved by hand, wave
+// priorities round the products and other orders of the workgroups made no difference.
 //
 // LDS.  A key row is a token's D fp16 numbers, a value row an element's of all tokens; both
 // are 16 bytes longer than that, and value rows move on by 16 more after every eight, so

@@ -251,6 +251,17 @@ def test_a_decode_batch_of_ragged_lengths(gpu, given):
     check_attention(gpu, lengths, queries, 8, 2, 128, 64, "bf16", given_starts=given)
 
 
+@pytest.mark.parametrize("Hq,H,D,window", [(32, 16, 64, 0), (16, 16, 128, 0), (32, 16, 64, 1100)])
+def test_many_long_sequences_in_equal_shares(gpu, Hq, H, D, window):
+    """More long sequences than workgroups for four parts of each: shares that begin and end
+    inside sequences, span short and empty ones, and are many or few."""
+    lengths = [1, 1500, 0, 40, 1100, 0, 2000, 3, 64, 1025, 17, 1030]
+    check_attention(gpu, lengths, [1 if n else 0 for n in lengths], Hq, H, D, 64, "fp16",
+                    window=window)
+    check_attention(gpu, lengths, [min(n, 1 + i % 8) for i, n in enumerate(lengths)], H, H, D, 16,
+                    "bf16", window=window)
+
+
 @pytest.mark.parametrize("window", [1, 7, 16, 100, 4096])
 def test_windows(gpu, window):
     check_attention(gpu, [1, 90, 400], [1, 1, 1], 4, 2, 128, 16, "fp16", window=window)
