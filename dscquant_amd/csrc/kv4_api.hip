@@ -34,6 +34,9 @@ int check_dtype(int dtype) {
   return DSCQ_OK;
 }
 
+// A window that no sequence reaches the end of is none.
+int64_t window_of(int64_t window) { return window > kKvMaxLength ? 0 : window; }
+
 // Tokens of one call: their workgroups fit a grid, their rows 64-bit offsets.
 constexpr int64_t kMaxTokens = int64_t{1} << 30;
 
@@ -122,7 +125,7 @@ int64_t dscq_kv_attention_workspace_bytes(int64_t B, int64_t Hq, int64_t H, int6
   if (int rc = check_attention(B, Hq, H, D, max_q, max_length, window)) return rc;
   if (B == 0 || max_q == 0) return 0;
   return kv_attention_workspace_bytes((int)D, (int)B, (int)Hq, (int)H, (int)max_q, max_length,
-                                      window);
+                                      window_of(window));
 }
 
 int dscq_kv_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype,
@@ -144,7 +147,7 @@ int dscq_kv_attention(const void* q, int64_t q_token_stride, int64_t q_head_stri
     return fail("kv attention: without starts every sequence has one query");
   if (!starts && T != B) return fail("kv attention: without starts there are B queries");
   const int64_t need = kv_attention_workspace_bytes((int)D, (int)B, (int)Hq, (int)H, (int)max_q,
-                                                    max_length, window);
+                                                    max_length, window_of(window));
   if (need && (!workspace || !aligned(workspace, 16) || workspace_bytes < need))
     return fail("kv attention: needs a 16-byte aligned workspace of %lld bytes", (long long)need);
   KvAttend a;
@@ -162,7 +165,7 @@ int dscq_kv_attention(const void* q, int64_t q_token_stride, int64_t q_head_stri
   a.max_q = (int32_t)max_q;
   a.max_length = max_length;
   a.scale = scale;
-  a.window = window;
+  a.window = window_of(window);
   a.out = out;
   a.lse = lse;
   return kv_attention(a, (int)D, dtype == DSCQ_BF16, workspace, static_cast<hipStream_t>(stream));

@@ -95,6 +95,12 @@ def test_c_workspace_query():
     assert L.dscq_kv_attention_workspace_bytes(1, 4, 2, 128, 0, 64, 0) == 0
     assert L.dscq_kv_attention_workspace_bytes(1, 4, 2, 128, 1, 0, 0) >= 0
     assert L.dscq_kv_attention_workspace_bytes(1, 5, 2, 128, 1, 64, 0) == -1
+    # Windows that no sequence fills, up to the largest number, plan as none does.
+    for max_q in (1, 100):
+        plain = L.dscq_kv_attention_workspace_bytes(2, 8, 2, 128, max_q, 100000, 0)
+        assert plain > 0
+        for window in ((1 << 28) + 1, (1 << 63) - 1):
+            assert L.dscq_kv_attention_workspace_bytes(2, 8, 2, 128, max_q, 100000, window) == plain
 
 
 def test_python_refuses_cpu_tensors_and_layouts():
