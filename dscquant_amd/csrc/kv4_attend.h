@@ -40,7 +40,9 @@ __device__ __forceinline__ Sequence sequence_of(const KvAttend& a, int b) {
 }
 
 // One past the last token that query i sees, and the first.
-__device__ __forceinline__ int row_end(const Sequence& s, int i) { return max(s.L - s.n + i + 1, 0); }
+__device__ __forceinline__ int row_end(const Sequence& s, int i) {
+  return max(s.L - s.n + i + 1, 0);
+}
 __device__ __forceinline__ int row_begin(const KvAttend& a, const Sequence& s, int i) {
   const int64_t b = (int64_t)(s.L - s.n + i + 1) - a.window;
   return a.window && b > 0 ? (int)b : 0;

@@ -112,10 +112,12 @@ struct Rows {
 
   // The rows of a sequence and key/value head h: their q, and what they see.
   template <typename T>
-  __device__ __forceinline__ void load(const KvAttend& a, const Sequence& s, int h, int G, int lane) {
+  __device__ __forceinline__ void load(const KvAttend& a, const Sequence& s, int h, int G,
+                                       int lane) {
     // A row past the last one is the last one over again; it is not stored.
     const int g = lane >> 4, row = min(lane & 15, s.n * G - 1), i = row / G;
-    const T* p = static_cast<const T*>(a.q) + (s.first + i) * a.q_ts + (h * G + row - i * G) * a.q_hs;
+    const T* p = static_cast<const T*>(a.q) + (s.first + i) * a.q_ts +
+                 (h * G + row - i * G) * a.q_hs;
     Raw<T> raw[D / 32];
 #pragma unroll
     for (int w = 0; w < D / 32; ++w) raw[w] = load_raw_at<T>(p, g * (D / 4) + 8 * w);
@@ -242,7 +244,8 @@ struct Rows {
   // computed the next one's codes are on their way, and the one's after it pages.  The body
   // stands once and the codes move from register to register: a second copy of it would cost
   // a short run more, in instructions fetched for the first time, than the moves do.
-  __device__ __forceinline__ void run(const Pages<D>& g, int first, int last, int stride, int lane) {
+  __device__ __forceinline__ void run(const Pages<D>& g, int first, int last, int stride,
+                                      int lane) {
     if (first >= last) return;
     Tile<D> a = load_tile<D>(g, place_of(g.places, 2 * first));
     Tile<D> b = load_tile<D>(g, place_of(g.places, 2 * first + 1));
@@ -541,7 +544,8 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attend_join_kernel(KvAttend a,
 Plan plan_of(int B, int Hq, int H, int max_q, int64_t max_length, int64_t window) {
   const int64_t rows = (int64_t)max_q * (Hq / H), cus = cu_count();
   const int64_t length =
-      std::min<int64_t>(window ? std::min(max_length, window + max_q - 1) : max_length, kKvMaxLength);
+      std::min<int64_t>(window ? std::min(max_length, window + max_q - 1) : max_length,
+                        kKvMaxLength);
   Plan p = {};
   p.chunks = 1;
   if (rows > 16) {

@@ -49,7 +49,9 @@ struct Layout {
   static constexpr int kStarts = kFactors + 4 * kTokens, kInverses = kStarts + 4 * kTokens;
   static constexpr int kAll = kInverses + 4 * kTokens;
 
-  static __host__ __device__ constexpr int value_row(int d) { return d * kValueRow + (d >> 3) * 16; }
+  static __host__ __device__ constexpr int value_row(int d) {
+    return d * kValueRow + (d >> 3) * 16;
+  }
 };
 
 // One wave's tile of the next tokens, between memory and LDS: the keys while the first half

@@ -1,6 +1,7 @@
 """The 4-bit paged key/value cache of an attention layer.
 
-    new_cache(pages, page_size, heads, head_dim, device) -> u8 [pages, heads, page_size, head_dim + 8]
+    new_cache(pages, page_size, heads, head_dim, device)
+                          -> u8 [pages, heads, page_size, head_dim + 8]
     append(cache, q, k, v, slots, ...)    a step's rows into their slots, q turned and rotated
     attention(cache, q, tables, ...)      a ragged batch's queries over their pages
     read(cache, slots, dtype)             cached tokens as 16-bit rows
@@ -224,6 +225,7 @@ def attention(cache: torch.Tensor, q: torch.Tensor, tables: torch.Tensor, length
             _lib.call("dscq_kv_attention", q.data_ptr(), strides[0], strides[1], _DTYPES[q.dtype],
                       T, Hq, cache.data_ptr(), pages, P, H, D, _lib.ptr(tables), width,
                       lengths.data_ptr(), None if starts is None else starts.data_ptr(), B, max_q,
-                      max_length, scale, window, out.data_ptr(), _lib.ptr(lse), _lib.ptr(ws), max(need, 0),
+                      max_length, scale, window, out.data_ptr(), _lib.ptr(lse), _lib.ptr(ws),
+                      max(need, 0),
                       _lib.stream(dev))
     return (out, lse) if return_lse else out
