@@ -54,6 +54,12 @@ struct Layout {
   }
 };
 
+// Words below fp32's smallest normal number are a scale of 0, as a cache holds where nothing
+// was stored: their rows are zeros.  Factors of scores below kLeastFactor are none, so that
+// logarithms of scales over them stay finite.
+constexpr uint32_t kLeastWord = 0x00800000u;
+constexpr float kLeastFactor = 0x1p-118f;
+
 // One wave's tile of the next tokens, between memory and LDS: the keys while the first half
 // of a step computes, the values during the second, so that one of them is in registers.
 template <int D, int NW>
@@ -95,20 +101,24 @@ struct Stage {
   __device__ __forceinline__ void store_keys(uint8_t* lds, int wave, int lane, float to2,
                                              int begin, int end, const Masks& masks) const {
     const int g = lane >> 4, t = wave * kKvTile + (lane & 15);
-    const ZeroPair z = zero_pair(kw, kw, masks);
+    // A key whose scores are 0 whatever its codes: zeros, with a factor that has a reciprocal.
+    const bool none = fabsf(__uint_as_float(kw) * to2) < kLeastFactor;
+    const uint32_t zero = none ? 0u : kw;
+    const ZeroPair z = zero_pair(zero, zero, masks);
 #pragma unroll
     for (int w = 0; w < D / 32; ++w) {
       h2 e[4];
-      unpack_word(codes.w[w], z, masks, e);
+      unpack_word(none ? 0u : codes.w[w], z, masks, e);
       *reinterpret_cast<h8*>(lds + t * L::kKeyRow + g * (D / 2) + w * 16) =
           join8(e[0], e[1], e[2], e[3]);
     }
     if (g == 0) {
       // The three numbers of a token.  A page that is not there: infinite scores, so that it
       // is noticed; a token outside the workgroup's: zeros (whoever looks there masks it);
-      // one whose value is not finite: NaN scores.
+      // one whose value is not finite: NaN scores; one whose value is zeros: as of scale 1.
       const int j = token + (lane & 15);
-      const float y = __uint_as_float(vw), f = __uint_as_float(kw) * to2;
+      const float y = vw < kLeastWord ? 1.0f : __uint_as_float(vw);
+      const float f = none ? 1.0f : __uint_as_float(kw) * to2;
       const bool in = j >= begin && j < end;
       const float start = __builtin_amdgcn_logf(y) * __builtin_amdgcn_rcpf(f);
       float* out = reinterpret_cast<float*>(lds + L::kFactors) + t;
@@ -121,12 +131,26 @@ struct Stage {
                                                const Masks& masks) const {
     const int c = chunk(lane), q = quad(lane);
     const int to = L::kKeys + L::value_row(c * (D / 16)) + wave * 32 + (q & 1) * 16 + (q >> 1) * 8;
-    const ZeroPair z[2] = {zero_pair(vq.x, vq.y, masks), zero_pair(vq.z, vq.w, masks)};
+    uint4 words = vq;
+    Words<D> from = codes;
+    const uint32_t least = min(min(vq.x, vq.y), min(vq.z, vq.w));
+    if (__builtin_amdgcn_ballot_w64(least < kLeastWord)) {
+      // Values of scale 0: zeros, whatever their codes (two tokens a word of codes).
+      const uint32_t keep[2] = {(vq.x < kLeastWord ? 0u : 0xFFFFu) |
+                                    (vq.y < kLeastWord ? 0u : 0xFFFF0000u),
+                                (vq.z < kLeastWord ? 0u : 0xFFFFu) |
+                                    (vq.w < kLeastWord ? 0u : 0xFFFF0000u)};
+      words = make_uint4(vq.x & keep[0], vq.y & (keep[0] >> 16), vq.z & keep[1],
+                         vq.w & (keep[1] >> 16));
+#pragma unroll
+      for (int m = 0; m < D / 32; ++m) from.w[m] &= keep[m / (D / 64)];
+    }
+    const ZeroPair z[2] = {zero_pair(words.x, words.y, masks), zero_pair(words.z, words.w, masks)};
 #pragma unroll
     for (int m = 0; m < D / 64; ++m) {
       h2 e[2][4];
-      unpack_word(codes.w[m], z[0], masks, e[0]);
-      unpack_word(codes.w[D / 64 + m], z[1], masks, e[1]);
+      unpack_word(from.w[m], z[0], masks, e[0]);
+      unpack_word(from.w[D / 64 + m], z[1], masks, e[1]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         typedef _Float16 h4 __attribute__((ext_vector_type(4)));

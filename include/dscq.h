@@ -370,7 +370,8 @@ int dscq_device_supported(void);
  *   A row x of D numbers: lo = min(x, 0), hi = max(x, 0), base = max((hi - lo) / 15, 1e-8)
  *   rounded up to a multiple of 16 last places, zero = round(-lo / base) in [0, 15],
  *   scale = base + zero last places, code = round(x / scale + zero) in [0, 15], standing for
- *   (code - zero) * scale; all in fp32.  A row that is not finite is stored as NaN.
+ *   (code - zero) * scale; all in fp32.  A row that is not finite is stored as NaN.  A word
+ *   of 0, as in memory of zeros where nothing was stored, is a row of zeros whatever its codes.
  * slot   page * page_size + place of a token; slots of one call are distinct.
  *
  * dscq_kv_append: the step's rows into their slots.

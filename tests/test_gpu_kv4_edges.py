@@ -1,0 +1,156 @@
+"""What attention over the 4-bit cache does at its edges, in each of its forms, against
+oracle/kv4.py in 64 bits.
+
+The bound.  With weights that carry a relative error of at most d an output is off by at most
+2 d sum p |v|.  d counts the rounding of a weight to the 11 bits of fp16 (once, 2^-11 in all,
+since the sum is of unrounded weights) and the fp32 scores (2^-12 for sum |q k| scale < 32, as
+these inputs have).  fp16's smallest numbers are 2^-24 apart and a part's largest weight times
+scale is held at 2^7 or above, so that each token may add half of 2^-24 2^-7 of that weight
+times scale for each of the up to 15 steps its value is from zero: L 15 2^-32.  Then the
+output's own rounding (fp16: half of 2^-24 at least).  Tokens without weight enter nowhere.
+"""
+import numpy as np
+import pytest
+import torch
+
+from dscquant_amd import kv4
+from oracle import kv4 as oracle
+from test_gpu_kv4 import DT, UNIT, f32, random_cache
+
+pytestmark = pytest.mark.gpu
+
+# Hq, H, sequences, queries of each, the host's bound on the length: what chooses the form.
+FORMS = {
+    "whole": (4, 2, 2, 3, 1000),
+    "parts": (4, 2, 2, 3, 5000),
+    "shares": (32, 32, 6, 3, 5000),
+    "prompt, 4 waves": (8, 2, 2, 20, 1000),
+    "prompt, 8 waves": (8, 2, 2, 40, 1000),
+}
+every_form = pytest.mark.parametrize("form", FORMS)
+
+
+class Batch:
+    """Sequences of random codes on pages of their own; ``k_words``, ``v_words`` [pages, H, P]
+    are the words of the cache's rows, changed before the first use."""
+
+    def __init__(self, form, dtype, D=128, P=16, L=300, seed=0):
+        self.Hq, self.H, self.B, n, self.max_length = FORMS[form]
+        self.dtype, self.D, self.P, self.counts = dtype, D, P, [n] * self.B
+        self.rng = np.random.default_rng(seed)
+        self.lengths = [L - 61 * (b % 3) for b in range(self.B)]
+        self.per = -(-L // P)
+        self.raw = random_cache(self.rng, self.B * self.per, self.H, P, D, 0.1)
+        at = P * D
+        flat = self.raw.reshape(self.B * self.per, self.H, -1)
+        self.k_words = flat[..., at:at + 4 * P].view("<u4")
+        self.v_words = flat[..., at + 4 * P:].view("<u4")
+        self.tables = np.arange(self.B * self.per, dtype=np.int32).reshape(self.B, -1)
+        T = sum(self.counts)
+        self.q = torch.randn(T, self.Hq, D, generator=torch.Generator().manual_seed(seed)).to(DT[dtype])
+
+    def words(self, which, b, j):
+        """The words [H] of sequence b's token j, as a view."""
+        return (self.k_words, self.v_words)[which][b * self.per + j // self.P, :, j % self.P]
+
+    def run(self, gpu, **options):
+        i32 = lambda a: torch.tensor(np.asarray(a, np.int32), device=gpu)  # noqa: E731
+        starts = np.concatenate(([0], np.cumsum(self.counts)))
+        options = {"max_q": max(self.counts), "max_length": self.max_length, **options}
+        out, lse = kv4.attention(torch.from_numpy(self.raw).to(gpu), self.q.to(gpu),
+                                 i32(self.tables), i32(self.lengths), i32(starts),
+                                 return_lse=True, **options)
+        return f32(out), f32(lse)
+
+    def expect(self, b, scale=None):
+        """(out, lse, bound) of sequence b's queries."""
+        k, v = (x[self.tables[b]].reshape(-1, self.H, self.D)[:self.lengths[b]].astype(np.float64)
+                for x in oracle.values(self.raw))
+        first, n, L = sum(self.counts[:b]), self.counts[b], self.lengths[b]
+        q = f32(self.q[first:first + n]).astype(np.float64)
+        scale = self.D ** -0.5 if scale is None else scale
+        out, lse, spread = oracle.attention(q, k, v, np.arange(L - n, L), scale)
+        f = self.v_words.view("<f4").astype(np.float64)[self.tables[b]].transpose(0, 2, 1)
+        f = f.reshape(-1, self.H)[:L]
+        G = self.Hq // self.H
+        most = np.zeros((n, self.Hq, 1))
+        for i in range(n):
+            for h in range(self.Hq):
+                seen = slice(0, L - n + i + 1)
+                w = np.exp(scale * (k[seen, h // G] @ q[i, h]) - lse[i, h])
+                most[i, h] = np.max(w * f[seen, h // G])
+        bound = (UNIT[self.dtype] * np.abs(out) + spread * 2.0 ** -10 + L * 15 * 2.0 ** -32 * most
+                 + (2.0 ** -25 if self.dtype == "fp16" else 0))
+        return out, lse, bound
+
+    def check(self, gpu, scale=None, **options):
+        have, have_lse = self.run(gpu, scale=scale, **options)
+        for b in range(self.B):
+            first = sum(self.counts[:b])
+            rows = slice(first, first + self.counts[b])
+            out, lse, bound = self.expect(b, scale)
+            # All zeros would not pass.
+            assert (np.abs(out) > 2 * bound)[np.isfinite(out)].mean() > 0.5
+            close(have[rows], out, bound)
+            close(have_lse[rows], lse, 2.0 ** -12 + np.abs(lse) * 2.0 ** -22)
+
+
+def close(have, want, bound):
+    """Elements that are not finite are the same; the others within the bound."""
+    finite = np.isfinite(want)
+    assert np.array_equal(have[~finite], want[~finite], equal_nan=True)
+    off = np.abs(have - want)[finite] - bound[finite]
+    assert (off <= 0).all(), float(off.max())
+
+
+# ------------------------------------------------------------------- tokens of scale 0
+
+@every_form
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("what", ["key", "value", "both"])
+def test_a_scale_of_zero_is_a_row_of_zeros(gpu, form, D, what):
+    """Whatever the codes: a key of zeros scores 0, a value of zeros keeps its weight.  Words
+    of less than fp32's smallest normal number are as good as 0."""
+    x = Batch(form, "fp16", D)
+    for b in range(x.B):
+        for j, word in ((0, 0), (17, 0), (18, 0), (100, 5), (x.lengths[b] - 5, 0)):
+            if what != "value":
+                x.words(0, b, j)[:] = word
+            if what != "key":
+                x.words(1, b, j)[:] = word
+    x.check(gpu)
+
+
+@every_form
+def test_all_values_zero(gpu, form):
+    """The results are 0 and the log sums are the scores'."""
+    x = Batch(form, "bf16")
+    x.v_words[:] = 0
+    out, lse = x.run(gpu)
+    assert (out == 0).all()
+    for b in range(x.B):
+        first = sum(x.counts[:b])
+        want = x.expect(b)[1]
+        close(lse[first:first + x.counts[b]], want, 2.0 ** -12 + np.abs(want) * 2.0 ** -22)
+
+
+@pytest.mark.parametrize("n", [1, 3, 12, 40])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_tokens_left_out_of_a_new_cache(gpu, n, dtype):
+    """A token whose slot is outside the cache stays a place of zeros that its sequence counts."""
+    L, D, P, Hq = 60, 64, 16, 4
+    g = torch.Generator().manual_seed(n)
+    q, k, v = (torch.randn(L, h, D, generator=g).to(DT[dtype]).to(gpu) for h in (Hq, 1, 1))
+    cache = kv4.new_cache(4, P, 1, D, gpu)
+    slots = torch.arange(L, device=gpu)
+    for j in (7, 33, L - 2):
+        slots[j] = -1
+    kv4.append(cache, None, k, v, slots)
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device=gpu)  # noqa: E731
+    out, lse = kv4.attention(cache, q[L - n:], i32([[0, 1, 2, 3]]), i32([L]), i32([0, n]), max_q=n,
+                             max_length=L, return_lse=True)
+    kk, vv = (x.reshape(-1, 1, D)[:L] for x in oracle.values(cache.cpu().numpy()))
+    assert (kk[7] == 0).all() and (vv[33] == 0).all()
+    want, sums, spread = oracle.attention(f32(q[L - n:]), kk, vv, np.arange(L - n, L), D ** -0.5)
+    close(f32(out), want, UNIT[dtype] * np.abs(want) + spread * 2.0 ** -10 + 2.0 ** -25)
+    close(f32(lse), sums, 2.0 ** -12 + np.abs(sums) * 2.0 ** -22)
