@@ -43,11 +43,13 @@ struct Layout {
   static constexpr int kTokens = 16 * NW, kSteps = kTokens / 32;
   static constexpr int kKeyRow = 2 * D + 16, kValueRow = 2 * kTokens + 16;  // bytes
   // A buffer (there are two): keys, values, and for each token three fp32 numbers: the
-  // factor of its scores, what they start from, and one over its value's scale.
+  // factor of its scores, what they start from, and one over its value's scale; then a word
+  // a tile, not 0 where one of its values is not finite.
   static constexpr int kKeys = kTokens * kKeyRow;
   static constexpr int kFactors = kKeys + D * kValueRow + D * 2;
   static constexpr int kStarts = kFactors + 4 * kTokens, kInverses = kStarts + 4 * kTokens;
-  static constexpr int kAll = kInverses + 4 * kTokens;
+  static constexpr int kBad = kInverses + 4 * kTokens;
+  static constexpr int kAll = kBad + 4 * NW;
 
   static __host__ __device__ constexpr int value_row(int d) {
     return d * kValueRow + (d >> 3) * 16;
@@ -112,19 +114,22 @@ struct Stage {
       *reinterpret_cast<h8*>(lds + t * L::kKeyRow + g * (D / 2) + w * 16) =
           join8(e[0], e[1], e[2], e[3]);
     }
+    const int j = token + (lane & 15);
+    const bool in = there && j >= begin && j < end;
+    const float y = vw < kLeastWord ? 1.0f : __uint_as_float(vw);
+    const bool bad = in && !(y > 0.0f);
+    const uint64_t any = __builtin_amdgcn_ballot_w64(bad);
+    if (lane == 0) *(reinterpret_cast<uint32_t*>(lds + L::kBad) + wave) = any != 0;
     if (g == 0) {
       // The three numbers of a token.  A page that is not there: infinite scores, so that it
       // is noticed; a token outside the workgroup's: zeros (whoever looks there masks it);
-      // one whose value is not finite: NaN scores; one whose value is zeros: as of scale 1.
-      const int j = token + (lane & 15);
-      const float y = vw < kLeastWord ? 1.0f : __uint_as_float(vw);
+      // one whose value is zeros: as of scale 1; is not finite: that, with the sign to tell.
       const float f = none ? 1.0f : __uint_as_float(kw) * to2;
-      const bool in = j >= begin && j < end;
       const float start = __builtin_amdgcn_logf(y) * __builtin_amdgcn_rcpf(f);
       float* out = reinterpret_cast<float*>(lds + L::kFactors) + t;
-      out[0] = !there ? INFINITY : in ? (y > 0.0f ? f : __uint_as_float(kKvNan)) : 0.0f;
-      out[L::kTokens] = !there ? INFINITY : in && y > 0.0f ? start : 0.0f;
-      out[2 * L::kTokens] = there && in && y > 0.0f ? __builtin_amdgcn_rcpf(y) : 0.0f;
+      out[0] = !there ? INFINITY : in ? f : 0.0f;
+      out[L::kTokens] = !there ? INFINITY : in && !bad ? start : 0.0f;
+      out[2 * L::kTokens] = bad ? -1.0f : in ? __builtin_amdgcn_rcpf(y) : 0.0f;
     }
   }
   __device__ __forceinline__ void store_values(uint8_t* lds, int wave, int lane,
@@ -206,6 +211,17 @@ struct Wave {
     return t;
   }
 
+  // Values of the buffer's tokens, from j0 on, that are not finite: the rows that see one are
+  // NaN from here on (the weights and their sum are not, so that log sums are the scores').
+  __device__ __forceinline__ void look(const uint8_t* lds, int j0) {
+    const float* r = reinterpret_cast<const float*>(lds + L::kInverses);
+    bool bad = false;
+#pragma unroll 1
+    for (int n = 0; n < L::kTokens; ++n) bad |= (r[n] < 0.0f) & (j0 + n >= lo) & (j0 + n < hi);
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) o[d] *= bad ? __uint_as_float(kKvNan) : 1.0f;
+  }
+
   // The tokens j0 .. j0 + 31, the sub-th of the buffer, with their products t; NEXT: then t
   // are the following ones, whose products run beside this softmax.
   template <bool NEXT>
@@ -255,7 +271,7 @@ struct Wave {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float e = __builtin_amdgcn_exp2f(s[4 * n + i]);
-        l = __builtin_fmaf(e, r[i], l);
+        l = __builtin_fmaf(e, fabsf(r[i]), l);
         p[n >> 1][4 * (n & 1) + i] = (_Float16)e;
       }
     }
@@ -360,7 +376,9 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_attend_prompt_kernel(KvAttend a
     if (more) stage.load_keys(a, block, page_bytes, place, NW * (at + 1) + wave, lane);
     place = place_of(places, NW * (at + 2) + wave);
     f16 t;
+    uint32_t bad = 0;  // of tile lane % NW
     if (work) {
+      bad = *reinterpret_cast<const uint32_t*>(now + L::kBad + 4 * (lane & (NW - 1)));
       t = w.scores(now, 0);
 #pragma unroll
       for (int sub = 0; sub < L::kSteps / 2; ++sub)
@@ -375,6 +393,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_attend_prompt_kernel(KvAttend a
       for (int sub = L::kSteps / 2; sub < L::kSteps - 1; ++sub)
         w.template step<true>(now, sub, j0 + 32 * sub, t);
       w.template step<false>(now, L::kSteps - 1, j0 + L::kTokens - 32, t);
+      if (__builtin_amdgcn_ballot_w64(bad != 0)) w.look(now, j0);
     }
     if (more) stage.store_values(next, wave, lane, masks);
     __syncthreads();

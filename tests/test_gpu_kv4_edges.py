@@ -154,3 +154,28 @@ def test_tokens_left_out_of_a_new_cache(gpu, n, dtype):
     want, sums, spread = oracle.attention(f32(q[L - n:]), kk, vv, np.arange(L - n, L), D ** -0.5)
     close(f32(out), want, UNIT[dtype] * np.abs(want) + spread * 2.0 ** -10 + 2.0 ** -25)
     close(f32(lse), sums, 2.0 ** -12 + np.abs(sums) * 2.0 ** -22)
+
+
+# ------------------------------------------------------------------- rows that are not finite
+
+@every_form
+@pytest.mark.parametrize("which", ["key", "value"])
+def test_a_row_that_is_not_finite_and_the_log_sum(gpu, form, which):
+    """Who sees a NaN value has a NaN result and the log sum of its scores; who sees a NaN key
+    has neither; who sees neither is not touched."""
+    x = Batch(form, "fp16", 64)
+    n = x.counts[0]
+    for b in range(x.B):
+        # One for the last query alone, in one head; in the second sequence for half of them.
+        j = x.lengths[b] - (1 if b != 1 else n // 2 + 1)
+        x.words(which == "value", b, j)[:1] = 0x7FC00000
+    have, have_lse = x.run(gpu)
+    for b in range(x.B):
+        first = sum(x.counts[:b])
+        out, lse, bound = x.expect(b)
+        sees = np.isnan(out).all(-1)
+        rows = 1 if b != 1 else n // 2 + 1
+        assert sees.sum() == rows * x.Hq // x.H and np.isnan(out).any(-1).sum() == sees.sum()
+        assert np.array_equal(np.isnan(lse), sees if which == "key" else np.zeros_like(sees))
+        close(have[first:first + n], out, np.where(np.isnan(out), 0, bound))
+        close(have_lse[first:first + n], lse, 2.0 ** -12 + np.abs(lse) * 2.0 ** -22)
