@@ -463,7 +463,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_attend_split_kernel(
 
 // A row's parts, weighted by their sums.  Grid: (max_q Hq, B) rows, one a wave, or (`per` = 4)
 // a workgroup, whose waves take every fourth part; eight at a time, so that their loads are
-// in flight together.
+// in flight together.  A part that is NaN makes its row NaN, whatever its weight.
 template <int D, typename T>
 __global__ __launch_bounds__(64 * kWaves) void kv_attend_join_kernel(KvAttend a, Shares shares,
                                                                      Plan plan, int per) {
@@ -515,7 +515,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attend_join_kernel(KvAttend a,
       const float p = c + m * per < used ? __builtin_amdgcn_exp2f(log[m] - base) : 0.0f;
       sum += p;
 #pragma unroll
-      for (int e = 0; e < kE; ++e) y[e] = p == 0.0f ? y[e] : __builtin_fmaf(p, x[m][e], y[e]);
+      for (int e = 0; e < kE; ++e) y[e] = __builtin_fmaf(p, x[m][e], y[e]);
     }
   }
   if (per > 1) {

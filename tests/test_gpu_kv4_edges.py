@@ -179,3 +179,22 @@ def test_a_row_that_is_not_finite_and_the_log_sum(gpu, form, which):
         assert np.array_equal(np.isnan(lse), sees if which == "key" else np.zeros_like(sees))
         close(have[first:first + n], out, np.where(np.isnan(out), 0, bound))
         close(have_lse[first:first + n], lse, 2.0 ** -12 + np.abs(lse) * 2.0 ** -22)
+
+
+@every_form
+def test_a_value_that_is_not_finite_far_below_the_rest(gpu, form):
+    """... is NaN to whoever sees it however small its weight, also as a part of its own."""
+    x = Batch(form, "bf16", 64, L=420)
+    x.q = x.q.abs()
+    for b in range(x.B):
+        for j in range(0, 260, x.P):  # whole pages of keys of -15 scale: scores some 200 below
+            page = b * x.per + j // x.P
+            x.raw.reshape(x.B * x.per, x.H, -1)[page, :, :x.P * x.D // 2] = 0
+            x.k_words[page] |= 15
+        x.words(1, b, 0)[:1] = 0x7FC00000
+    have, have_lse = x.run(gpu, scale=2.0)
+    for b in range(x.B):
+        rows = slice(sum(x.counts[:b]), sum(x.counts[:b + 1]))
+        out, lse, _ = x.expect(b, scale=2.0)
+        assert np.isnan(out).any() and np.array_equal(np.isnan(have[rows]), np.isnan(out))
+        assert (np.abs(have_lse[rows] - lse) <= 2.0 ** -6 + np.abs(lse) * 2.0 ** -22).all()
