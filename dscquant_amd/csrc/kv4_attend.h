@@ -22,10 +22,11 @@ __device__ __forceinline__ int32_t uniform_load(const int32_t* p) {
   return *(Ptr)(reinterpret_cast<uintptr_t>(p));
 }
 
-// Sequence b's queries (rows first .. first + n - 1 of q) and length.
+// Sequence b's queries (rows first .. first + n - 1 of q) and the first one's place among its
+// tokens, less than 0 where it has more queries than tokens.  max_q cuts n off, not the places.
 struct Sequence {
   int64_t first;
-  int n, L;
+  int n, place;
 };
 __device__ __forceinline__ Sequence sequence_of(const KvAttend& a, int b) {
   int64_t s0 = b, s1 = b + 1;
@@ -33,18 +34,19 @@ __device__ __forceinline__ Sequence sequence_of(const KvAttend& a, int b) {
     s0 = max(uniform_load(a.starts + b), 0);
     s1 = uniform_load(a.starts + b + 1);
   }
+  const int64_t L = min((int64_t)max(uniform_load(a.lengths + b), 0), a.width * a.cache.P);
+  const int place = (int)(L - max(s1 - s0, 0));
   s0 = min(s0, a.T);
   s1 = min(max(s1, s0), a.T);
-  const int64_t L = min((int64_t)max(uniform_load(a.lengths + b), 0), a.width * a.cache.P);
-  return {s0, (int)min(s1 - s0, (int64_t)a.max_q), (int)L};
+  return {s0, (int)min(s1 - s0, (int64_t)a.max_q), place};
 }
 
 // One past the last token that query i sees, and the first.
 __device__ __forceinline__ int row_end(const Sequence& s, int i) {
-  return max(s.L - s.n + i + 1, 0);
+  return max(s.place + i + 1, 0);
 }
 __device__ __forceinline__ int row_begin(const KvAttend& a, const Sequence& s, int i) {
-  const int64_t b = (int64_t)(s.L - s.n + i + 1) - a.window;
+  const int64_t b = (int64_t)(s.place + i + 1) - a.window;
   return a.window && b > 0 ? (int)b : 0;
 }
 

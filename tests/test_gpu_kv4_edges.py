@@ -62,21 +62,22 @@ class Batch:
                                  return_lse=True, **options)
         return f32(out), f32(lse)
 
-    def expect(self, b, scale=None):
+    def expect(self, b, scale=None, window=0):
         """(out, lse, bound) of sequence b's queries."""
         k, v = (x[self.tables[b]].reshape(-1, self.H, self.D)[:self.lengths[b]].astype(np.float64)
                 for x in oracle.values(self.raw))
         first, n, L = sum(self.counts[:b]), self.counts[b], self.lengths[b]
         q = f32(self.q[first:first + n]).astype(np.float64)
         scale = self.D ** -0.5 if scale is None else scale
-        out, lse, spread = oracle.attention(q, k, v, np.arange(L - n, L), scale)
+        out, lse, spread = oracle.attention(q, k, v, np.arange(L - n, L), scale, window)
         f = self.v_words.view("<f4").astype(np.float64)[self.tables[b]].transpose(0, 2, 1)
         f = f.reshape(-1, self.H)[:L]
         G = self.Hq // self.H
         most = np.zeros((n, self.Hq, 1))
         for i in range(n):
             for h in range(self.Hq):
-                seen = slice(0, L - n + i + 1)
+                end = L - n + i + 1
+                seen = slice(max(end - window, 0) if window else 0, end)
                 w = np.exp(scale * (k[seen, h // G] @ q[i, h]) - lse[i, h])
                 most[i, h] = np.max(w * f[seen, h // G])
         bound = (UNIT[self.dtype] * np.abs(out) + spread * 2.0 ** -10 + L * 15 * 2.0 ** -32 * most
@@ -198,3 +199,21 @@ def test_a_value_that_is_not_finite_far_below_the_rest(gpu, form):
         out, lse, _ = x.expect(b, scale=2.0)
         assert np.isnan(out).any() and np.array_equal(np.isnan(have[rows]), np.isnan(out))
         assert (np.abs(have_lse[rows] - lse) <= 2.0 ** -6 + np.abs(lse) * 2.0 ** -22).all()
+
+
+# ------------------------------------------------------------------- bounds and rows
+
+@every_form
+@pytest.mark.parametrize("window", [0, 40])
+def test_queries_past_max_q_leave_the_others_in_their_places(gpu, form, window):
+    x = Batch(form, "fp16", 64)
+    n = x.counts[0]
+    x.counts[1] = 1  # one that is not cut off
+    x.q = x.q[:sum(x.counts)]
+    for max_q in (n - 1, n - n // 8 - 1):
+        have, have_lse = x.run(gpu, max_q=max_q, window=window)
+        for b in range(x.B):
+            first, m = sum(x.counts[:b]), min(x.counts[b], max_q)
+            out, lse, bound = x.expect(b, window=window)
+            close(have[first:first + m], out[:m], bound[:m])
+            close(have_lse[first:first + m], lse[:m], 2.0 ** -12 + np.abs(lse[:m]) * 2.0 ** -22)
