@@ -15,6 +15,8 @@ typedef float f16 __attribute__((ext_vector_type(16)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+// The binary place that a row's largest weight times scale is given, and may pass by eight.
+constexpr float kReference = 7.0f;
 
 // A value every lane holds alike, read through the scalar cache.
 __device__ __forceinline__ int32_t uniform_load(const int32_t* p) {

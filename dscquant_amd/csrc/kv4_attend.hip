@@ -21,10 +21,11 @@
 //
 // Weights.  p'_j = 2^((s_j - m) log2 e + x) f'_j for the value's scale f', rounded to fp16 (the
 // one rounding here that is not fp32's: 2^-11 of a weight, the size of an fp16 output's own),
-// and the sum is that of 2^((s_j - m) log2 e + x) in fp32.  The exponent x keeps the largest
-// f' 2^x in [2^6, 2^7), and m lags the true maximum by up to 8 binary places, so weights are at
-// most 2^15: within fp16, and its small numbers end 2^39 below.  While neither has to move
-// (a vote of the wave) a step rescales nothing.
+// and the sum is that of 2^((s_j - m) log2 e + x) in fp32.  The row's reference x - m follows
+// its largest weight times scale, which it puts at 2^7 and which may pass that by 8 binary
+// places before the reference moves: within fp16, whose small numbers end 2^31 below.  A value
+// without weight moves nothing, however large.  A step whose largest score and largest scale
+// together stay below the limit (a vote of the wave) rescales nothing.
 //
 // This file: up to sixteen rows a key/value head (single tokens, a few drafted ones), bound by
 // the cache's bytes, D + 8 a token and head.  A step of a wave is 32 tokens, 4352 bytes at
@@ -52,6 +53,9 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kStep = 2 * kKvTile;  // tokens of a step
+// What a scale below it counts as where the reference is chosen: values of zeros have weights
+// too, whose sum stays within fp32 this way.  (The rule's least scale is 2^-27.)
+constexpr float kLeastScale = 0x1p-32f;
 
 // What a lane reads of a 16-token tile.
 template <int D>
@@ -105,8 +109,7 @@ template <int D>
 struct Rows {
   h8 q[D / 32];
   f4 o[D / 16];                                   // o[t][i]: element (4 g + i) D/16 + t
-  float off = 0.0f, limit = -INFINITY, l = 0.0f;  // x less the maximum; what moves it; the sum
-  float x = 0.0f, value_limit = 0.0f;             // the values' exponent, the scale that moves it
+  float off = 0.0f, limit = -INFINITY, l = 0.0f;  // the reference; what moves it; the sum
   float to2;                                      // scores to binary places: scale log2 e 2^-k
   int begin, end, all_begin, all_end;             // the row's tokens; those that every row sees
 
@@ -191,25 +194,19 @@ struct Rows {
     }
     const float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])),
                             fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-    float most = fmaxf(fmaxf(fmaxf(vf[0], vf[1]), fmaxf(vf[2], vf[3])),
-                       fmaxf(fmaxf(vf[4], vf[5]), fmaxf(vf[6], vf[7])));
-    if (__builtin_amdgcn_ballot_w64((top > limit) | (most > value_limit))) {
-      float shift = 0.0f;
-      // Rows can differ in what they see, so the largest scale is the wave's.
+    float most = kLeastScale;
 #pragma unroll
-      for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
-      if (most > value_limit) {
-        const int e = __builtin_amdgcn_frexp_expf(most);
-        shift = (float)(7 - e) - x;
-        x = (float)(7 - e);
-        value_limit = __builtin_amdgcn_ldexpf(1.0f, e);
-      }
-      // A row whose largest score passed its limit gets it as the new maximum.
-      const float high = row_max(top);
-      const bool up = high > limit, fresh = limit == -INFINITY;
-      const float delta = up ? x - high : shift;
-      const float keep = fresh ? 0.0f : __builtin_amdgcn_exp2f(delta);
-      limit = up || !fresh ? x + 8.0f : limit;
+    for (int i = 0; i < 8; ++i) most = fmaxf(most, vf[i]);
+    if (__builtin_amdgcn_ballot_w64(top + __builtin_amdgcn_logf(most) > limit)) {
+      float high = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        high = fmaxf(high, s[i] + __builtin_amdgcn_logf(fmaxf(vf[i], kLeastScale)));
+      high = row_max(high);
+      const bool up = high > limit;
+      const float delta = up ? kReference - high : 0.0f;
+      const float keep = limit == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(delta);
+      limit = up ? kReference + 8.0f : limit;
       off += delta;
       l *= keep;
 #pragma unroll

@@ -166,9 +166,6 @@ struct Stage {
   }
 };
 
-// The binary place that a row's largest weight is given, and may pass by eight.
-constexpr float kReference = 7.0f;
-
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
 
 // The running state of a wave's 32 rows.

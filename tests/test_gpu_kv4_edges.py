@@ -217,3 +217,32 @@ def test_queries_past_max_q_leave_the_others_in_their_places(gpu, form, window):
             out, lse, bound = x.expect(b, window=window)
             close(have[first:first + m], out[:m], bound[:m])
             close(have_lse[first:first + m], lse[:m], 2.0 ** -12 + np.abs(lse[:m]) * 2.0 ** -22)
+
+
+# ------------------------------------------------------------------- scales of values
+
+@every_form
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("places", [16, 20, 24, 28, 40])
+def test_a_large_value_without_weight_changes_nothing(gpu, form, dtype, places):
+    """Values 2^places times the others' whose scores lie some 100 below (weights of 2^-140):
+    the first tokens, ones in the middle, and one that the last query alone sees."""
+    x = Batch(form, dtype, 64)
+    x.q = x.q.abs()
+    byte = oracle.places(x.P, x.D)[0][0]
+    flat = x.raw.reshape(x.B * x.per, x.H, -1)
+    for b in range(x.B):
+        for j in (0, 1, 130, x.lengths[b] - 1):
+            flat[b * x.per + j // x.P][:, byte[j % x.P]] = 0  # a key of -15
+            x.words(0, b, j)[:] = np.float32(1).view(np.uint32) | 15
+            x.words(1, b, j)[:] += np.uint32(places << 23)
+    x.check(gpu)
+
+
+@every_form
+@pytest.mark.parametrize("D", [64, 128])
+def test_values_of_all_sizes(gpu, form, D):
+    """Scales from 2^-26 to 2^40, weights as they come."""
+    x = Batch(form, "bf16", D)
+    x.v_words += (x.rng.integers(-24, 42, x.v_words.shape) << 23).astype(np.uint32)
+    x.check(gpu)
