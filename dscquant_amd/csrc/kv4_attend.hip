@@ -10,9 +10,9 @@
 //
 // Products.  A key is k = (c - z) f with whole numbers c, z in [0, 15] and the row's scale f:
 // q . k = f (q . (c - z)), and c - z is exact in fp16, so keys and values enter the products
-// as what they are.  q enters as fp16; a bf16 q is first multiplied by the power of two that
+// as what they are.  q enters as fp16; a bf16 row is first multiplied by the power of two that
 // takes its largest element to [2^14, 2^15) (eight bits of each element, so exact but for
-// elements 2^38 times smaller than the row's largest).  Both products are made transposed,
+// elements 2^31 times smaller than the row's largest).  Both products are made transposed,
 //   S^T = K q^T  (16 tokens x 16 rows),  O^T += V^T P^T  (16 elements x 16 rows),
 // because then a lane holds scores of one row only -- lane (c, g) = (lane % 16, lane / 16)
 // those of row c and tokens 4 g .. 4 g + 3 of a tile -- so maximum, sum and rescaling are
@@ -139,8 +139,7 @@ struct Rows {
 #pragma unroll
         for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(y[e]));
       }
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+      top = row_max(top);
       if (top > 0.0f && top < INFINITY) k = min(15 - __builtin_amdgcn_frexp_expf(top), 60);
     }
     to2 = __builtin_amdgcn_ldexpf(a.scale * kLog2e, -k);

@@ -4,8 +4,10 @@
 // bound the time, and next to them the softmax (an exponential and four other operations a
 // score) and the unpacking, so the codes are unpacked once for a workgroup: its four or
 // eight waves take 64 or 128 tokens in turn, a 16-token tile each, and leave keys and values
-// as fp16 in LDS (twice, so that the next tokens are written while these are used); every
-// wave multiplies all of them with 32 rows of its own, which it holds in registers.
+// in LDS (twice, so that the next tokens are written while these are used), values as fp16 and
+// keys in the queries' type, which holds their whole numbers exactly and is then the queries'
+// own: every wave multiplies all of them with 32 rows of its own, as they are, which it holds
+// in registers.
 // 32 x 32 x 16 products: S^T (32 tokens x 32 rows) leaves lane (c, h) = (lane % 32, lane / 32)
 // the scores of row c and tokens 8 a + 4 h + i, which as they lie are the operand of
 // O^T += V^T P^T over the token order 16 s + 4 h + 0..3, 16 s + 8 + 4 h + 0..3; V^T is stored
@@ -26,7 +28,7 @@
 // reads a product) do not fit its registers: 6.1 ms.  Instructions interleaved by hand, wave
 // priorities round the products and other orders of the workgroups made no difference.
 //
-// LDS.  A key row is a token's D fp16 numbers, a value row an element's of all tokens; both
+// LDS.  A key row is a token's D 16-bit numbers, a value row an element's of all tokens; both
 // are 16 bytes longer than that, and value rows move on by 16 more after every eight, so
 // that the eight lanes that read or write 16 bytes together (and the sixteen that write 8)
 // meet all banks, and a lane's places differ by constants.
@@ -56,6 +58,31 @@ struct Layout {
   }
 };
 
+// Eight numbers as a product with rows of type T takes them; whole numbers of fp16 so.
+template <typename T>
+struct Operand {
+  typedef h8 V;
+  static __device__ __forceinline__ V of(const h2 e[4]) { return join8(e[0], e[1], e[2], e[3]); }
+  static __device__ __forceinline__ f16 mfma(V a, V b, f16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Operand<bf16> {
+  typedef __bf16 V __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ V of(const h2 e[4]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)  // the upper halves of two fp32 numbers
+      w[i] = __builtin_amdgcn_perm(__float_as_uint((float)e[i][1]), __float_as_uint((float)e[i][0]),
+                                   0x07060302u);
+    return __builtin_bit_cast(V, make_uint4(w[0], w[1], w[2], w[3]));
+  }
+  static __device__ __forceinline__ f16 mfma(V a, V b, f16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+
 // Words below fp32's smallest normal number are a scale of 0, as a cache holds where nothing
 // was stored: their rows are zeros.  Factors of scores below kLeastFactor are none, so that
 // logarithms of scales over them stay finite.
@@ -64,9 +91,10 @@ constexpr float kLeastFactor = 0x1p-118f;
 
 // One wave's tile of the next tokens, between memory and LDS: the keys while the first half
 // of a step computes, the values during the second, so that one of them is in registers.
-template <int D, int NW>
+template <int D, typename T, int NW>
 struct Stage {
   using L = Layout<D, NW>;
+  using V = typename Operand<T>::V;
   Words<D> codes;
   uint32_t kw, vw;  // the words of token lane % 16
   uint4 vq;         // the values' words of the quad
@@ -111,8 +139,7 @@ struct Stage {
     for (int w = 0; w < D / 32; ++w) {
       h2 e[4];
       unpack_word(none ? 0u : codes.w[w], z, masks, e);
-      *reinterpret_cast<h8*>(lds + t * L::kKeyRow + g * (D / 2) + w * 16) =
-          join8(e[0], e[1], e[2], e[3]);
+      *reinterpret_cast<V*>(lds + t * L::kKeyRow + g * (D / 2) + w * 16) = Operand<T>::of(e);
     }
     const int j = token + (lane & 15);
     const bool in = there && j >= begin && j < end;
@@ -169,10 +196,11 @@ struct Stage {
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
 
 // The running state of a wave's 32 rows.
-template <int D, int NW>
+template <int D, typename T, int NW>
 struct Wave {
   using L = Layout<D, NW>;
-  h8 q[D / 16];
+  using V = typename Operand<T>::V;
+  V q[D / 16];
   f16 o[D / 32];
   float off = 0.0f, limit = -INFINITY, l = 0.0f;  // less the reference; what moves it; the sum
   int lo, hi, all_lo, all_hi;                     // the row's tokens; those of all rows
@@ -199,9 +227,8 @@ struct Wave {
     }
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
-      const h8 k =
-          *reinterpret_cast<const h8*>(lds + key_at + sub * 32 * L::kKeyRow + ks * 32);
-      t = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[ks], t, 0, 0, 0);
+      const V k = *reinterpret_cast<const V*>(lds + key_at + sub * 32 * L::kKeyRow + ks * 32);
+      t = Operand<T>::mfma(k, q[ks], t);
       // Not all keys in registers at once.
       if (ks == D / 32 - 1) asm volatile("" ::: "memory");
     }
@@ -289,7 +316,6 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_attend_prompt_kernel(KvAttend a
                                                                       int groups, int least) {
   using L = Layout<D, NW>;
   __shared__ alignas(16) uint8_t lds[2 * L::kAll];
-  __shared__ float tops[NW];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 31, h = lane >> 5;
   const int b = blockIdx.y, H = a.cache.H;
@@ -309,7 +335,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_attend_prompt_kernel(KvAttend a
   if (blockIdx.z > 0 && from >= last) return;
 
   // The wave's rows: tokens that some see, and that all see.
-  Wave<D, NW> w;
+  Wave<D, T, NW> w;
   w.clear(lane);
   const int r0 = g0 + wave * 32, row = r0 + c, i = min(row, count - 1) / G;
   const int i0 = min(r0, count - 1) / G, i1 = (min(r0 + 32, count) - 1) / G;
@@ -319,43 +345,18 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_attend_prompt_kernel(KvAttend a
   w.lo = row_begin(a, s, i);
   w.hi = row_end(s, i);
 
-  // q as fp16, the workgroup's largest element in [2^14, 2^15) (bf16; fp16 as it is).
   const T* qrow = static_cast<const T*>(a.q) + (s.first + i) * a.q_ts +
                   (head * G + min(row, count - 1) - i * G) * a.q_hs;
-  Raw<T> raw[D / 16];
 #pragma unroll
-  for (int ks = 0; ks < D / 16; ++ks) raw[ks] = load_raw_at<T>(qrow, 16 * ks + 8 * h);
-  int k = 0;
-  if constexpr (std::is_same<T, bf16>::value) {
-    float top = 0.0f, y[8];
-#pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) {
-      to_f32(raw[ks], y);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(y[e]));
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-    if (lane == 0) tops[wave] = top;
-    __syncthreads();
-#pragma unroll
-    for (int x = 0; x < NW; ++x) top = fmaxf(top, tops[x]);
-    if (top > 0.0f && top < INFINITY) k = min(15 - __builtin_amdgcn_frexp_expf(top), 60);
-  }
-#pragma unroll
-  for (int ks = 0; ks < D / 16; ++ks) {
-    float y[8];
-    to_f32(raw[ks], y);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) w.q[ks][e] = (_Float16)__builtin_amdgcn_ldexpf(y[e], k);
-  }
-  const float to2 = __builtin_amdgcn_ldexpf(a.scale * kLog2e, -k);
+  for (int ks = 0; ks < D / 16; ++ks)
+    w.q[ks] = __builtin_bit_cast(typename Operand<T>::V, load_raw_at<T>(qrow, 16 * ks + 8 * h).w);
+  const float to2 = a.scale * kLog2e;
 
   const uint8_t* const block = a.cache.data + head * kv_block_bytes<D>(a.cache.P);
   const int64_t page_bytes = H * kv_block_bytes<D>(a.cache.P);
   const Places places = places_of(a, b, end);
   const Masks masks;
-  Stage<D, NW> stage;
+  Stage<D, T, NW> stage;
   if (from < to) {
     stage.load_keys(a, block, page_bytes, place_of(places, NW * from + wave), NW * from + wave,
                     lane);

@@ -246,3 +246,58 @@ def test_values_of_all_sizes(gpu, form, D):
     x = Batch(form, "bf16", D)
     x.v_words += (x.rng.integers(-24, 42, x.v_words.shape) << 23).astype(np.uint32)
     x.check(gpu)
+
+
+# ------------------------------------------------------------------- queries of all sizes
+
+@every_form
+@pytest.mark.parametrize("dtype,size", [("fp16", 1.0), ("bf16", 1.0), ("bf16", 2.0 ** 20)])
+@pytest.mark.parametrize("factor", [2.0 ** 12, 2.0 ** 34, 2.0 ** 100, 2.0 ** -40, float("inf"), float("nan")])
+def test_a_query_does_not_depend_on_the_others(gpu, form, dtype, size, factor):
+    """One head of one query far larger or smaller than the rest, infinite or NaN: the other
+    rows are what they are without it, bit for bit."""
+    x = Batch(form, dtype, 64)
+    x.q *= size
+    scale = 0.125 / size
+    plain, plain_lse = x.run(gpu, scale=scale)
+    assert np.isfinite(plain).all()
+    others = np.ones((x.q.shape[0], x.Hq), bool)
+    n = x.counts[0]
+    for row, head in ((0, x.Hq - 1), (n + n // 2, 0)):
+        x.q[row, head] *= factor
+        others[row, head] = False
+    have, have_lse = x.run(gpu, scale=scale)
+    assert np.array_equal(have[others], plain[others])
+    assert np.array_equal(have_lse[others], plain_lse[others])
+    if np.isnan(factor):
+        assert np.isnan(have[~others]).all() and np.isnan(have_lse[~others]).all()
+    if factor == 2.0 ** -40:  # scores of 0: the mean of what it sees
+        for b, head in ((0, x.Hq - 1), (1, 0)):
+            out, lse, bound = x.expect(b, scale)
+            i = b * (n // 2)
+            close(have[b * n + i, head], out[i, head], bound[i, head])
+            close(have_lse[b * n + i, head], lse[i, head], np.array(2.0 ** -12 + 8 * 2.0 ** -22))
+
+
+@every_form
+@pytest.mark.parametrize("size", [2.0 ** -60, 2.0 ** -30, 2.0 ** 30, 2.0 ** 60])
+def test_queries_of_one_size_and_a_scale_that_undoes_it(gpu, form, size):
+    """bf16 queries of any size: each element counts with its eight bits."""
+    x = Batch(form, "bf16", 128)
+    x.q *= size
+    x.check(gpu, scale=128 ** -0.5 / size)
+
+
+@every_form
+def test_elements_of_a_query_far_apart(gpu, form):
+    """Elements 2^25 times the others that meet keys of zeros there: what is left counts in full."""
+    x = Batch(form, "bf16", 64)
+    byte, shift = oracle.places(x.P, x.D)[0]
+    flat = x.raw.reshape(x.B * x.per, x.H, -1)
+    d = 5
+    for t in range(x.P):  # the code of element d is its zero-point
+        zero = (x.k_words[..., t] & 15).astype(np.uint8)
+        at, s = byte[t, d], int(shift[t, d])
+        flat[..., at] = (flat[..., at] & np.uint8(255 ^ 15 << s)) | zero << np.uint8(s)
+    x.q[..., d] *= 2.0 ** 25
+    x.check(gpu)
