@@ -141,13 +141,18 @@ int dscq_kv_attention(const void* q, int64_t q_token_stride, int64_t q_head_stri
   if (!(T >= 0 && T <= kMaxTokens && width >= 0 && width <= kKvMaxLength / page_size))
     return fail("kv attention: invalid dimensions");
   if (!(scale > 0.0f && scale < 3.0e38f)) return fail("kv attention: scale must be positive");
-  if (T == 0 || B == 0 || max_q == 0) return DSCQ_OK;
-  if (!q || !lengths || !out || (width && !tables)) return fail("kv attention: null buffer");
-  if (!starts && max_q != 1)
+  if (T == 0) return DSCQ_OK;
+  const bool none = B == 0 || max_q == 0;
+  if (!out || (!none && (!q || !lengths || (width && !tables))))
+    return fail("kv attention: null buffer");
+  if (!none && !starts && max_q != 1)
     return fail("kv attention: without starts every sequence has one query");
-  if (!starts && T != B) return fail("kv attention: without starts there are B queries");
-  const int64_t need = kv_attention_workspace_bytes((int)D, (int)B, (int)Hq, (int)H, (int)max_q,
-                                                    max_length, window_of(window));
+  if (!none && !starts && T != B)
+    return fail("kv attention: without starts there are B queries");
+  const int64_t need = none ? 0
+                            : kv_attention_workspace_bytes((int)D, (int)B, (int)Hq, (int)H,
+                                                           (int)max_q, max_length,
+                                                           window_of(window));
   if (need && (!workspace || !aligned(workspace, 16) || workspace_bytes < need))
     return fail("kv attention: needs a 16-byte aligned workspace of %lld bytes", (long long)need);
   KvAttend a;

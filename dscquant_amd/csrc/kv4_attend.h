@@ -29,10 +29,14 @@ __device__ __forceinline__ int32_t uniform_load(const int32_t* p) {
 struct Sequence {
   int64_t first;
   int n, place;
+  int64_t past;     // queries past max_q
+  int64_t lo, hi;  // the rows of all sequences (loaded here so that one wait is enough)
 };
 __device__ __forceinline__ Sequence sequence_of(const KvAttend& a, int b) {
-  int64_t s0 = b, s1 = b + 1;
+  int64_t s0 = b, s1 = b + 1, lo = 0, hi = a.T;
   if (a.starts) {
+    lo = min(max(uniform_load(a.starts), 0), a.T);
+    hi = max(uniform_load(a.starts + a.B), 0);
     s0 = max(uniform_load(a.starts + b), 0);
     s1 = uniform_load(a.starts + b + 1);
   }
@@ -40,7 +44,8 @@ __device__ __forceinline__ Sequence sequence_of(const KvAttend& a, int b) {
   const int place = (int)(L - max(s1 - s0, 0));
   s0 = min(s0, a.T);
   s1 = min(max(s1, s0), a.T);
-  return {s0, (int)min(s1 - s0, (int64_t)a.max_q), place};
+  const int n = (int)min(s1 - s0, (int64_t)a.max_q);
+  return {s0, n, place, s1 - s0 - n, lo, hi};
 }
 
 // One past the last token that query i sees, and the first.
@@ -50,6 +55,29 @@ __device__ __forceinline__ int row_end(const Sequence& s, int i) {
 __device__ __forceinline__ int row_begin(const KvAttend& a, const Sequence& s, int i) {
   const int64_t b = (int64_t)(s.place + i + 1) - a.window;
   return a.window && b > 0 ? (int)b : 0;
+}
+
+// Rows that nothing is computed for, of no sequence or past max_q: results 0, log sums -inf.
+// Every step-th of the rows from r0 to r1 - 1, by the threads of a workgroup.
+__device__ __forceinline__ void clear_rows(const KvAttend& a, int D, int64_t r0, int64_t r1,
+                                           int64_t step, int threads) {
+  const int row = a.Hq * D;
+#pragma unroll 1
+  for (int64_t r = r0; r < r1; r += step) {
+    uint16_t* out = static_cast<uint16_t*>(a.out) + r * row;
+    for (int e = threadIdx.x * 8; e < row; e += threads * 8)
+      *reinterpret_cast<u32x4_a2*>(out + e) = (u32x4_a2){0, 0, 0, 0};
+    for (int h = threadIdx.x; a.lse && h < a.Hq; h += threads) a.lse[r * a.Hq + h] = -INFINITY;
+  }
+}
+// The rows before the first sequence's and after the last one's, dealt out to all workgroups.
+__device__ __forceinline__ void clear_outside(const KvAttend& a, const Sequence& s, int D,
+                                              int threads) {
+  if (s.lo == 0 && s.hi >= a.T) return;
+  const int64_t all = (int64_t)gridDim.x * gridDim.y * gridDim.z;
+  const int64_t mine = ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
+  clear_rows(a, D, mine, s.lo, all, threads);
+  clear_rows(a, D, s.hi + mine, a.T, all, threads);
 }
 
 struct Part {  // rows' results over some of their tokens

@@ -386,7 +386,10 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_attend_split_kernel(
   if constexpr (FORM != kShares) {
     const int b = blockIdx.z, h = blockIdx.y;
     const Sequence s = sequence_of(a, b);
+    clear_outside(a, s, D, 64 * NW);
     if (s.n <= 0) return;
+    if (s.past && blockIdx.x == 0)
+      clear_rows(a, D, s.first + s.n + h, s.first + s.n + s.past, a.cache.H, 64 * NW);
     const Steps steps = steps_of(a, s);
     int from = steps.first, to = from + steps.count;
     int64_t slot = -1;
@@ -401,6 +404,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_attend_split_kernel(
                            FORM == kParts ? plan.chunks : 0);
     return;
   }
+  clear_outside(a, sequence_of(a, 0), D, 64 * NW);
   // Where in the batch's steps this workgroup's share begins: the steps of all sequences,
   // summed by the threads, a run of sequences each.
   __shared__ int64_t wave_sums[NW];
@@ -447,7 +451,11 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_attend_split_kernel(
     if (steps.count == 0) continue;
     const int64_t end = start + steps.count;
     const int64_t part0 = start / share, used = (end - 1) / share - part0 + 1;
-    if (h == 0 && at == start && t == 0) shares.where[b] = {(int)part0 + b, (int)used};
+    if (at == start) {
+      if (h == 0 && t == 0) shares.where[b] = {(int)part0 + b, (int)used};
+      if (s.past)
+        clear_rows(a, D, s.first + s.n + h, s.first + s.n + s.past, a.cache.H, 64 * NW);
+    }
     const int s0 = __builtin_amdgcn_readfirstlane((int)(at - start));
     const int s1 = __builtin_amdgcn_readfirstlane((int)(min(to, end) - start));
     attend_steps<D, T, NW>(a, shares, joint, s, b, h, steps.first + s0, steps.first + s1,
@@ -535,6 +543,11 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attend_join_kernel(KvAttend a,
     o[e] = __builtin_bit_cast(uint16_t, to_out<T>(sum == 0.0f ? 0.0f : y[e] / sum));
   if (a.lse && lane == 0)
     a.lse[to] = sum == 0.0f ? -INFINITY : (base + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
+// No sequences, or no queries of them: every row is one that nothing is computed for.
+__global__ __launch_bounds__(64 * kWaves) void kv_attend_none_kernel(KvAttend a, int D) {
+  clear_rows(a, D, blockIdx.x, a.T, gridDim.x, 64 * kWaves);
 }
 
 Plan plan_of(int B, int Hq, int H, int max_q, int64_t max_length, int64_t window) {
@@ -637,6 +650,11 @@ int64_t kv_attention_workspace_bytes(int D, int B, int Hq, int H, int max_q, int
 }
 
 int kv_attention(const KvAttend& a, int D, bool is_bf16, void* ws, hipStream_t stream) {
+  if (a.B == 0 || a.max_q == 0) {
+    launch(kv_attend_none_kernel, dim3((uint32_t)std::min<int64_t>(a.T, 8 * cu_count())),
+           dim3(64 * kWaves), stream, a, D);
+    return launch_status("kv_attention");
+  }
   if (D == 128)
     return is_bf16 ? attend<128, bf16>(a, ws, stream) : attend<128, __half>(a, ws, stream);
   return is_bf16 ? attend<64, bf16>(a, ws, stream) : attend<64, __half>(a, ws, stream);

@@ -323,6 +323,9 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_attend_prompt_kernel(KvAttend a
   const int head = blockIdx.x % H, group = groups - 1 - blockIdx.x / H, chunks = gridDim.z;
   const int G = a.Hq / H;
   const Sequence s = sequence_of(a, b);
+  clear_outside(a, s, D, 64 * NW);
+  if (s.past && group == 0 && blockIdx.z == 0)
+    clear_rows(a, D, s.first + s.n + head, s.first + s.n + s.past, H, 64 * NW);
   const int count = s.n * G, g0 = group * (32 * NW);
   if (g0 >= count) return;
 

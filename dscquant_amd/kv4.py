@@ -187,9 +187,9 @@ def attention(cache: torch.Tensor, q: torch.Tensor, tables: torch.Tensor, length
     sequence.  ``max_q`` and ``max_length`` (default: what the tables hold) bound a
     sequence's queries and length on the host, which plans the launch by them.  ``scale``
     defaults to D ** -0.5; ``window`` > 0: a query sees that many tokens, its own the last.
-    A query that sees none gives zeros.  ``return_lse``: also the logarithm of each
-    query's softmax sum, fp32 [T, Hq] (-inf for one that sees none), with which results over
-    parts of a context are joined."""
+    A query that sees none gives zeros, and so do rows of no sequence and queries past
+    ``max_q``.  ``return_lse``: also the logarithm of each query's softmax sum, fp32 [T, Hq]
+    (-inf for one that sees none), with which results over parts of a context are joined."""
     pages, H, P, D = _check_cache(cache)
     index = cache.get_device()
     T, Hq = q.size(0), _heads("q", q, D)
@@ -216,7 +216,7 @@ def attention(cache: torch.Tensor, q: torch.Tensor, tables: torch.Tensor, length
     _lib.require_gfx950(dev)
     out = q.new_empty((T, Hq, D))
     lse = q.new_empty((T, Hq), dtype=torch.float32) if return_lse else None
-    if T and B and max_q:
+    if T:
         with _lib.on(dev):
             # The plan, and with it the scratch, depends on the device's compute units.
             need = int(_lib.lib().dscq_kv_attention_workspace_bytes(B, Hq, H, D, max_q, max_length,

@@ -413,9 +413,10 @@ int dscq_kv_read(const uint8_t* cache, int64_t pages, int64_t page_size, int64_t
  *   tables   i32 [B, width]: the pages of each sequence, in order; tokens of a page outside
  *            the cache are not seen.
  *   lengths  i32 [B]; at most width * page_size tokens are seen.
- *   starts   i32 [B + 1], or NULL: one query a sequence (T = B, max_q = 1).
+ *   starts   i32 [B + 1], not falling, or NULL: one query a sequence (T = B, max_q = 1).  Rows
+ *            of q before starts[0] and from starts[B] on are of no sequence and see no token.
  *   max_q, max_length  bounds of a sequence's queries and length known to the host: queries
- *            past max_q are not computed; longer lengths are, less evenly.
+ *            past max_q see no token; longer lengths are computed, less evenly.
  *   out      [T, Hq, D] of q's type; lse f32 [T, Hq] (natural logarithm) or NULL.
  *   workspace  16-byte aligned scratch of dscq_kv_attention_workspace_bytes (may be 0).
  * Limits: Hq a multiple of H up to 4096, B <= 65535, max_q Hq < 2^31, width * page_size <=

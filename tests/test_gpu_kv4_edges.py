@@ -301,3 +301,70 @@ def test_elements_of_a_query_far_apart(gpu, form):
         flat[..., at] = (flat[..., at] & np.uint8(255 ^ 15 << s)) | zero << np.uint8(s)
     x.q[..., d] *= 2.0 ** 25
     x.check(gpu)
+
+
+# ------------------------------------------------------------------- rows of no sequence
+
+@pytest.fixture
+def dirty(monkeypatch):
+    """Results are allocated with NaN in them."""
+    empty = torch.Tensor.new_empty
+    monkeypatch.setattr(torch.Tensor, "new_empty",
+                        lambda *a, **k: empty(*a, **k).fill_(float("nan")))
+
+
+@every_form
+@pytest.mark.parametrize("before,after,cut", [(0, 3, 0), (2, 0, 0), (5, 700, 0), (0, 0, 1), (1, 2, 2)])
+def test_rows_of_no_sequence_see_nothing(gpu, dirty, form, before, after, cut):
+    """Rows before the first sequence's, after the last one's and past max_q: 0 and -inf."""
+    x = Batch(form, "fp16", 64, L=140)
+    n, T = x.counts[0], sum(x.counts)
+    starts = before + np.arange(x.B + 1) * n
+    i32 = lambda a: torch.tensor(np.asarray(a, np.int32), device=gpu)  # noqa: E731
+    q = torch.cat((torch.full((before, x.Hq, 64), 7.0), x.q.float(),
+                   torch.full((after, x.Hq, 64), float("nan")))).to(x.q.dtype)
+    args = (torch.from_numpy(x.raw).to(gpu), q.to(gpu), i32(x.tables), i32(x.lengths), i32(starts))
+    kw = dict(max_q=n - cut, max_length=x.max_length)
+    out, lse = (f32(t) for t in kv4.attention(*args, return_lse=True, **kw))
+    assert np.array_equal(f32(kv4.attention(*args, **kw)), out)
+    row = np.arange(before + T + after) - before
+    none = (row < 0) | (row >= T) | (row % n >= n - cut)
+    assert (out[none] == 0).all() and (lse[none] == -np.inf).all()
+    for b in range(x.B):
+        want, sums, bound = x.expect(b)
+        m = n - cut
+        close(out[starts[b]:starts[b] + m], want[:m], bound[:m])
+        close(lse[starts[b]:starts[b] + m], sums[:m], 2.0 ** -12 + np.abs(sums[:m]) * 2.0 ** -22)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_rows_without_sequences_or_queries(gpu, dirty, dtype):
+    cache = kv4.new_cache(2, 16, 2, 64, gpu)
+    q = torch.full((300, 6, 64), float("nan"), device=gpu).to(DT[dtype])
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device=gpu)  # noqa: E731
+    for B, max_q in ((0, 5), (2, 0), (0, 0), (2, 5), (2, 70)):
+        out, lse = kv4.attention(cache, q, i32(B, 1), i32(B), i32(B + 1), max_q=max_q,
+                                 return_lse=True)
+        assert (out == 0).all() and (lse == -float("inf")).all(), (B, max_q)
+        assert (kv4.attention(cache, q, i32(B, 1), i32(B), i32(B + 1), max_q=max_q) == 0).all()
+
+
+def test_rows_of_no_sequence_in_many_short_ones(gpu, dirty):
+    """A padded batch in equal shares: sequences of no tokens, of no queries, of more than max_q."""
+    H, D, P = 64, 64, 16
+    cache = torch.from_numpy(random_cache(np.random.default_rng(0), 8, H, P, D)).to(gpu)
+    counts = [0, 2, 0, 5, 1, 0, 3, 0]
+    lengths = [0, 3, 9, 16, 0, 0, 2, 16]
+    starts = np.concatenate(([4], 4 + np.cumsum(counts)))
+    T = int(starts[-1]) + 9
+    i32 = lambda a: torch.tensor(np.asarray(a, np.int32), device=gpu)  # noqa: E731
+    q = torch.randn(T, H, D, generator=torch.Generator().manual_seed(0)).half().to(gpu)
+    out, lse = kv4.attention(cache, q, i32(np.arange(8)[:, None]), i32(lengths), i32(starts),
+                             max_q=2, max_length=5000, return_lse=True)
+    assert torch.isfinite(out).all()
+    seen = np.zeros(T, bool)
+    for b, n in enumerate(counts):
+        for i in range(min(n, 2)):
+            seen[starts[b] + i] = lengths[b] - n + i >= 0
+    assert np.array_equal(np.isfinite(f32(lse)).all(-1), seen)
+    assert (f32(out)[~seen] == 0).all() and (f32(lse)[~seen] == -np.inf).all()
