@@ -37,7 +37,7 @@ int check_dtype(int dtype) {
 // A window that no sequence reaches the end of is none.
 int64_t window_of(int64_t window) { return window > kKvMaxLength ? 0 : window; }
 
-// Tokens of one call: their workgroups fit a grid, their rows 64-bit offsets.
+// Tokens of one call, in as many launches as they take.
 constexpr int64_t kMaxTokens = int64_t{1} << 30;
 
 int check_attention(int64_t B, int64_t Hq, int64_t heads, int64_t D, int64_t max_q,

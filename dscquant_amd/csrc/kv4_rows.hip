@@ -13,6 +13,8 @@
 // waiting for its row), one token of 32 heads in 4.0; 16384 tokens of 8 heads read back in
 // 16.8 us (85 MB, 5.1 TB/s, the rate of a large copy).
 
+#include <algorithm>
+
 #include "kv4.h"
 #include "mma_int4.h"
 #include "rowquant.h"
@@ -280,6 +282,23 @@ int heads_per_group(int64_t tiles, int heads) {
   return (int)((heads + groups - 1) / groups);
 }
 
+// Tokens of a launch: a grid that holds 2^32 threads or more (2^28 tokens of D = 128) is not
+// refused but wraps, so more tokens than this take several launches.
+constexpr int64_t kLaunchTokens = int64_t{1} << 27;
+
+// `launch(first, n)` for ranges of T tokens; timing events, if armed, span all of them.
+template <typename F>
+int in_launches(int64_t T, F launch) {
+  if (T <= kLaunchTokens) return launch(0, T);
+  const KernelEvents ev = take_kernel_events();
+  for (int64_t t = 0; t < T; t += kLaunchTokens) {
+    const int64_t n = std::min(kLaunchTokens, T - t);
+    arm_kernel_events({t == 0 ? ev.start : nullptr, t + n == T ? ev.stop : nullptr});
+    if (int rc = launch(t, n)) return rc;
+  }
+  return 0;
+}
+
 template <int D, typename T>
 int append_rows(const KvAppend& a, bool rotate, hipStream_t stream) {
   const int64_t tiles = (a.T + kRowThreads / (D / 8) - 1) / (kRowThreads / (D / 8));
@@ -308,19 +327,36 @@ int read_rows(const KvRead& a, bool rotate, hipStream_t stream) {
 }  // namespace
 
 int kv_append(const KvAppend& a, int D, bool is_bf16, bool rotate, hipStream_t stream) {
-  if (D == 128)
-    return is_bf16 ? append_rows<128, bf16>(a, rotate, stream)
-                   : append_rows<128, __half>(a, rotate, stream);
-  return is_bf16 ? append_rows<64, bf16>(a, rotate, stream)
-                 : append_rows<64, __half>(a, rotate, stream);
+  return in_launches(a.T, [&](int64_t first, int64_t n) {
+    KvAppend p = a;  // rows of 16-bit elements
+    p.T = n;
+    if (a.q) p.q = static_cast<const uint16_t*>(a.q) + first * a.q_ts;
+    p.k = static_cast<const uint16_t*>(a.k) + first * a.k_ts;
+    p.v = static_cast<const uint16_t*>(a.v) + first * a.v_ts;
+    if (a.cos) p.positions = a.positions + first;
+    p.slots = a.slots + first;
+    if (a.q) p.q_out = static_cast<uint16_t*>(a.q_out) + first * a.Hq * D;
+    if (D == 128)
+      return is_bf16 ? append_rows<128, bf16>(p, rotate, stream)
+                     : append_rows<128, __half>(p, rotate, stream);
+    return is_bf16 ? append_rows<64, bf16>(p, rotate, stream)
+                   : append_rows<64, __half>(p, rotate, stream);
+  });
 }
 
 int kv_read(const KvRead& a, int D, bool is_bf16, bool rotate, hipStream_t stream) {
-  if (D == 128)
-    return is_bf16 ? read_rows<128, bf16>(a, rotate, stream)
-                   : read_rows<128, __half>(a, rotate, stream);
-  return is_bf16 ? read_rows<64, bf16>(a, rotate, stream)
-                 : read_rows<64, __half>(a, rotate, stream);
+  return in_launches(a.T, [&](int64_t first, int64_t n) {
+    KvRead p = a;  // rows of 16-bit elements
+    p.T = n;
+    p.slots = a.slots + first;
+    p.k = static_cast<uint16_t*>(a.k) + first * a.cache.H * D;
+    p.v = static_cast<uint16_t*>(a.v) + first * a.cache.H * D;
+    if (D == 128)
+      return is_bf16 ? read_rows<128, bf16>(p, rotate, stream)
+                     : read_rows<128, __half>(p, rotate, stream);
+    return is_bf16 ? read_rows<64, bf16>(p, rotate, stream)
+                   : read_rows<64, __half>(p, rotate, stream);
+  });
 }
 
 }  // namespace dscq

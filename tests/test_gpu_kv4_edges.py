@@ -368,3 +368,39 @@ def test_rows_of_no_sequence_in_many_short_ones(gpu, dirty):
             seen[starts[b] + i] = lengths[b] - n + i >= 0
     assert np.array_equal(np.isfinite(f32(lse)).all(-1), seen)
     assert (f32(out)[~seen] == 0).all() and (f32(lse)[~seen] == -np.inf).all()
+
+
+# ------------------------------------------------------------------- more tokens than a launch
+
+def test_append_of_more_tokens_than_a_launch_holds(gpu):
+    """2^28 tokens of 128 elements and a few more (all of them one row in memory), of which those
+    at the ends of launches are kept."""
+    D, T = 128, (1 << 28) + 5
+    x = torch.randn(3, 1, D, device=gpu).half()
+    q, k, v = (x[i:i + 1].expand(T, 1, D) for i in range(3))
+    kept = [0, 1, (1 << 27) - 1, 1 << 27, (1 << 28) - 16, (1 << 28) - 1, 1 << 28, T - 1]
+    slots = torch.full((T,), -1, dtype=torch.int64, device=gpu)
+    slots[torch.tensor(kept, device=gpu)] = torch.arange(len(kept), device=gpu) + 5
+    cache, want = (kv4.new_cache(1, 16, 1, D, gpu) for _ in range(2))
+    kv4.append(cache, None, k, v, slots)
+    n = len(kept)
+    kv4.append(want, None, k[:n], v[:n], torch.arange(n, device=gpu) + 5)
+    assert torch.equal(cache, want) and want.any()
+
+
+def test_read_of_more_tokens_than_a_launch_holds(gpu):
+    D, T = 128, (1 << 28) + 5
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 160 << 30:
+        pytest.skip("needs 160 GB of free device memory")
+    cache = kv4.new_cache(1, 16, 1, D, gpu)
+    x = torch.randn(16, 1, D, device=gpu).half()
+    kv4.append(cache, None, x, x + 1, torch.arange(16, device=gpu))
+    slots = (torch.arange(T, device=gpu) * 7) % 16
+    want = kv4.read(cache, torch.arange(16, device=gpu))
+    got = kv4.read(cache, slots)
+    for a, b in zip(got, want):
+        for first in (0, (1 << 27) - 50, (1 << 28) - 50, T - 50):
+            assert torch.equal(a[first:first + 50], b[slots[first:first + 50]])
+    del got, a
+    torch.cuda.empty_cache()
