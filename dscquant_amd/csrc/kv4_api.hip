@@ -1,6 +1,8 @@
 // extern "C" entry points of the 4-bit key/value cache (declared in include/dscq.h):
 // argument checks, then asynchronous launches on the caller's stream.
 
+#include <algorithm>
+
 #include "../../include/dscq.h"
 #include "kv4.h"
 
@@ -36,6 +38,10 @@ int check_dtype(int dtype) {
 
 // A window that no sequence reaches the end of is none.
 int64_t window_of(int64_t window) { return window > kKvMaxLength ? 0 : window; }
+
+// Rows (query, head) of a sequence: twice as many threads, and a workgroup's more a key/value
+// head, make less than 2^32.
+constexpr int64_t kMaxRows = (int64_t{1} << 31) - (int64_t{1} << 20);
 
 // Tokens of one call, in as many launches as they take.
 constexpr int64_t kMaxTokens = int64_t{1} << 30;
@@ -138,7 +144,8 @@ int dscq_kv_attention(const void* q, int64_t q_token_stride, int64_t q_head_stri
   if (int rc = check_dtype(dtype)) return rc;
   if (int rc = check_cache(cache, pages, page_size, H, D)) return rc;
   if (int rc = check_attention(B, Hq, H, D, max_q, max_length, window)) return rc;
-  if (!(T >= 0 && T <= kMaxTokens && width >= 0 && width <= kKvMaxLength / page_size))
+  if (!(T >= 0 && T <= kMaxTokens && width >= 0 && width <= kKvMaxLength / page_size &&
+        std::min(max_q, T) * Hq <= kMaxRows))
     return fail("kv attention: invalid dimensions");
   if (!(scale > 0.0f && scale < 3.0e38f)) return fail("kv attention: scale must be positive");
   if (T == 0) return DSCQ_OK;

@@ -33,6 +33,8 @@
 // that the eight lanes that read or write 16 bytes together (and the sixteen that write 8)
 // meet all banks, and a lane's places differ by constants.
 
+#include <algorithm>
+
 #include "kv4_attend.h"
 
 namespace dscq {
@@ -436,7 +438,8 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_attend_prompt_kernel(KvAttend a
 template <int D, typename T>
 int prompt_typed(const KvAttend& a, const Part& part, int waves, int chunks, int least,
                  hipStream_t stream) {
-  const int64_t rows = (int64_t)a.max_q * (a.Hq / a.cache.H), per = 32 * waves;
+  // max_q may be far above what there is, and a grid of 2^32 threads wraps.
+  const int64_t rows = std::min<int64_t>(a.max_q, a.T) * (a.Hq / a.cache.H), per = 32 * waves;
   const int groups = (int)((rows + per - 1) / per);
   const dim3 grid((uint32_t)(groups * a.cache.H), a.B, chunks);
   if (waves == 8)

@@ -419,8 +419,8 @@ int dscq_kv_read(const uint8_t* cache, int64_t pages, int64_t page_size, int64_t
  *            past max_q see no token; longer lengths are computed, less evenly.
  *   out      [T, Hq, D] of q's type; lse f32 [T, Hq] (natural logarithm) or NULL.
  *   workspace  16-byte aligned scratch of dscq_kv_attention_workspace_bytes (may be 0).
- * Limits: Hq a multiple of H up to 4096, B <= 65535, max_q Hq < 2^31, width * page_size <=
- * 2^28, scale > 0.
+ * Limits: Hq a multiple of H up to 4096, B <= 65535, max_q Hq < 2^31, min(max_q, T) Hq <=
+ * 2^31 - 2^20, width * page_size <= 2^28, scale > 0.
  */
 int64_t dscq_kv_attention_workspace_bytes(int64_t B, int64_t Hq, int64_t H, int64_t D,
                                           int64_t max_q, int64_t max_length, int64_t window);

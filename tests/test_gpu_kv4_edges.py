@@ -404,3 +404,9 @@ def test_read_of_more_tokens_than_a_launch_holds(gpu):
             assert torch.equal(a[first:first + 50], b[slots[first:first + 50]])
     del got, a
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("form", ["prompt, 4 waves", "prompt, 8 waves"])
+def test_a_bound_on_the_queries_far_above_them(gpu, form):
+    x = Batch(form, "fp16", 64, L=140)
+    x.check(gpu, max_q=((1 << 31) - 1) // x.Hq)

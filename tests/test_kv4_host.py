@@ -179,3 +179,13 @@ def test_oracle_cache_round_trip_and_rows_that_are_not_finite():
     assert np.isnan(got_k[0, 1]).all() and np.isfinite(got_k[0, 0]).all()
     changed = (cache != before).reshape(3, 2, -1).sum()
     assert 0 < changed <= 3 * 2 * (64 + 8)
+
+
+def test_c_attention_of_more_rows_than_a_launch_holds():
+    """A grid of 2^32 threads wraps: refused.  A large max_q alone is a bound and no row."""
+    message = "kv attention: invalid dimensions"
+    rows = dict(Hq=2, starts=B16, max_q=(1 << 30) - 1, max_length=64)
+    assert _einval(*_attention(T=1 << 30, **rows)) == message
+    assert _einval(*_attention(T=(1 << 30) - (1 << 19) + 1, **rows)) == message
+    name, *args = _attention(T=0, **rows)
+    assert getattr(_lib.lib(), name)(*args) == 0
