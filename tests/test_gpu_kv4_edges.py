@@ -410,3 +410,66 @@ def test_read_of_more_tokens_than_a_launch_holds(gpu):
 def test_a_bound_on_the_queries_far_above_them(gpu, form):
     x = Batch(form, "fp16", 64, L=140)
     x.check(gpu, max_q=((1 << 31) - 1) // x.Hq)
+
+
+@pytest.mark.parametrize("T,Hq,H,D,P,R,interleaved,rotate,dtype", [
+    (9000, 7, 3, 128, 64, 128, False, True, "bf16"),   # groups of 4 heads
+    (20000, 5, 5, 64, 16, 32, True, False, "fp16"),    # of 4, and of 2 read back
+    (20000, 0, 6, 64, 16, 64, False, True, "fp16"),    # no queries: of 3, and of 2
+    (33001, 2, 2, 128, 128, 0, False, True, "fp16"),   # all heads one after another
+])
+def test_append_and_read_of_prompts_are_bit_exact(gpu, T, Hq, H, D, P, R, interleaved, rotate, dtype):
+    """Enough tokens that a workgroup takes several heads one after another, from q to k to v."""
+    g = torch.Generator().manual_seed(T + Hq)
+    rows = torch.randn(T, Hq + 2 * H, D, generator=g)
+    rows[..., 5] *= 30
+    rows = rows.to(DT[dtype])
+    q, k, v = rows[:, :Hq], rows[:, Hq:Hq + H], rows[:, Hq + H:]
+    on = rows.to(gpu)
+    pages = -(-T // P) + 1
+    slots = np.random.default_rng(T).permutation(pages * P)[:T]
+    slots[T // 3] = -1
+    at = torch.from_numpy(slots).to(gpu)
+    turned, options = lambda x: f32(x), {}  # noqa: E731
+    if R:
+        angle = torch.rand(500, R // 2, generator=g) * 6
+        pos = torch.randint(0, 500, (T,), generator=g)
+        c, s = angle.cos(), angle.sin()
+        turned = lambda x: oracle.turn(f32(x), c[pos].numpy(), s[pos].numpy(), interleaved)  # noqa: E731
+        options = dict(positions=pos.to(gpu), cos=c.to(gpu), sin=s.to(gpu), interleaved=interleaved)
+    cache = torch.full((pages, H, P, D + 8), 0xA5, dtype=torch.uint8, device=gpu)
+    got = kv4.append(cache, on[:, :Hq] if Hq else None, on[:, Hq:Hq + H], on[:, Hq + H:], at,
+                     rotate=rotate, **options)
+    qn, kn, vn = turned(q), turned(k), f32(v)
+    if rotate:
+        qn, kn = oracle.hadamard(qn) * np.float32(1 / D), oracle.hadamard(kn)
+    if Hq:
+        assert np.array_equal(f32(got), f32(torch.from_numpy(qn).to(DT[dtype])))
+    empty = np.full((pages, H, P, D + 8), 0xA5, np.uint8)
+    kept = slots >= 0
+    have = oracle.values(cache.cpu().numpy())
+    back = kv4.read(cache, at, DT[dtype], rotate=rotate)
+    for which, x in enumerate((kn, vn)):
+        codes, words = oracle.quantize(x)
+        stored = (codes.astype(np.float32) - (words & 15).astype(np.float32)[..., None]) \
+            * words.view(np.float32)[..., None]
+        want = oracle.values(empty)[which].reshape(pages * P, H, D)
+        want[slots[kept]] = stored[kept]
+        assert np.array_equal(have[which].reshape(pages * P, H, D), want)
+        if rotate and which == 0:
+            stored = oracle.hadamard(stored) * np.float32(1 / D)
+        stored[~kept] = 0
+        assert np.array_equal(f32(back[which]), f32(torch.from_numpy(stored).to(DT[dtype])))
+
+
+@every_form
+@pytest.mark.parametrize("D", [64, 128])
+def test_the_least_scales(gpu, form, D):
+    """Keys and values about the rule's least scale, 1e-8: results of 1e-7, which bf16 holds as
+    it holds others."""
+    x = Batch(form, "bf16", D)
+    x.v_words -= np.uint32(24 << 23)
+    x.k_words -= np.uint32(23 << 23)
+    assert x.v_words.view("<f4").min() < 1e-8 and x.k_words.view("<f4").min() < 1e-8
+    x.check(gpu, scale=2.0 ** 23 * D ** -0.5)
+    x.check(gpu)  # scores of 0 or so
