@@ -31,8 +31,8 @@
 // the cache's bytes, D + 8 a token and head.  A step of a wave is 32 tokens, 4352 bytes at
 // D = 128, for 240 vector instructions (160 of them unpack) and 16 matrix ones, which two
 // waves on a SIMD issue in 1.1 us together.  Measured (D = 128): 131072 tokens of 8 heads
-// (143 MB) 31.5 us and 5.7 for the join, 4.5 TB/s (a large copy here: 5.2); 64 sequences of 1
-// to 4096 tokens (143 MB) 45.5 and 5.7; 777 tokens of 32 heads 9.9, where start and end are 5.
+// (143 MB) 31.8 us and 5.2 for the join, 4.5 TB/s (a large copy here: 5.2); 64 sequences of 1
+// to 4096 tokens (143 MB) 45.4 and 5.6; 777 tokens of 32 heads 9.6, where start and end are 5.
 // More rows: kv4_prompt.hip.
 //
 // Measured and not kept: codes as fp16 subnormals, which the matrix cores take as they are
@@ -573,7 +573,8 @@ Plan plan_of(int B, int Hq, int H, int max_q, int64_t max_length, int64_t window
   p.rows = 16;
   p.step = kStep;
   // Up to 1024 tokens by the eight waves of one workgroup: four steps a wave cost less than
-  // the second kernel (8 sequences of 1000 tokens, 64/8 heads: 11.5 us, 14.0 split).
+  // the second kernel (8 sequences of 1000 tokens, 64/8 heads: 10.2 us, 13.3 in parts; one of
+  // 777, 32/32 heads: 8.7 and 9.9).
   p.form = length <= 1024 ? kWhole : kParts;
   p.waves = p.form == kWhole ? 8 : kWaves;
   if (p.form == kWhole) return p;
@@ -582,7 +583,8 @@ Plan plan_of(int B, int Hq, int H, int max_q, int64_t max_length, int64_t window
   // four of them a sequence or more, parts are a sequence's own; with fewer, a ragged batch
   // would leave most of the device waiting for its longest (64 sequences of 1 to 4096
   // tokens: 57 us in two parts each, 46 in equal shares), but a share that spans two
-  // sequences begins and ends twice (8 sequences of 2000: 20 us, 17 in parts).
+  // sequences begins and ends twice (17 sequences of 2000 in shares: 21.6 us; 16 in parts:
+  // 16.1).
   p.wgs = (int)std::max<int64_t>(1, 2 * cus / H);
   p.least = kWaves;
   if (B > p.wgs / 4) {

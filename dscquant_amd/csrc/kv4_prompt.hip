@@ -19,11 +19,11 @@
 // follows the row's largest t, which may pass it by eight binary places before it moves.
 //
 // Measured: 4096 queries after 12288 tokens, 64 query and 8 key/value heads of 128, bf16:
-// 1.96 ms (980 TFLOP/s of 4 D operations a visible pair; a large library product of the
-// type reaches 1190).  The matrix pipes are busy 44% of the cycles, a third of that beside
-// vector instructions (2.0 GHz under this load).  Without its exponentials the kernel would
+// 1.97 ms (980 TFLOP/s of 4 D operations a visible pair; a large library product of the
+// type reaches 1190).  The matrix pipes are busy 43% of the cycles, a third of that beside
+// vector instructions (2.1 GHz under this load).  Without its exponentials the kernel would
 // take 3% less, without reading values from LDS 2%, without unpacking 4%, with an eighth of
-// either product 20%.  2048 queries of 32 heads, fp16: 70 us (490 TFLOP/s): 256 workgroups,
+// either product 20%.  2048 queries of 32 heads, fp16: 72 us (480 TFLOP/s): 256 workgroups,
 // the longest of them 64 steps of 1.2 us one after another.  64 rows a wave (half the LDS
 // reads a product) do not fit its registers: 6.1 ms.  Instructions interleaved by hand, wave
 // priorities round the products and other orders of the workgroups made no difference.

@@ -13,7 +13,7 @@ kept at 4 bits by the rule of its activations (core/quantization.py:13-21), a sc
 zero-point for each row of a head: (head_dim + 8) / (4 head_dim) of their 16-bit size.
 Layout, rule and limits: include/dscq.h.  Keys and values enter the products as the whole
 numbers their codes stand for, so attention reads the cache as it is and rounds nothing of
-it.  Kernels run on torch's current stream; outputs and scratch come from torch's
+it; the softmax's weights enter theirs as fp16.  Kernels run on torch's current stream; outputs and scratch come from torch's
 allocator, so the calls can be captured in a HIP graph.  There is no gradient: the cache
 serves inference, as the integer linear path does.
 """
@@ -108,7 +108,8 @@ def append(cache: torch.Tensor, q, k: torch.Tensor, v: torch.Tensor, slots: torc
 
     ``q`` [T, Hq, D] (or None: None is returned), ``k``, ``v`` [T, H, D]: fp16 or bf16, each
     head's elements contiguous, any strides above (parts of one q|k|v product).  ``slots``
-    int64 [T], distinct; a slot outside the cache leaves its token out.  With ``cos``,
+    int64 [T], distinct; a slot outside the cache leaves its token out (a place of a new cache
+    that nothing was stored in is a key and a value of zeros to who sees it).  With ``cos``,
     ``sin`` (fp32 [rows, R / 2], R a multiple of 16 up to D) the first R elements of each
     head of q and k are turned by the row ``positions`` (int64 [T]) names: pairs
     (i, i + R / 2), or (2 i, 2 i + 1) if ``interleaved``.  A position outside the table:

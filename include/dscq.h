@@ -406,8 +406,10 @@ int dscq_kv_read(const uint8_t* cache, int64_t pages, int64_t page_size, int64_t
  * Causal attention of a ragged batch over the cache: sequence b's queries are rows
  * starts[b] .. starts[b + 1] - 1 of q, the last of its lengths[b] cached tokens; the query
  * at place p sees the tokens j <= p (and j > p - window where window > 0).
- *   out = softmax(scale q k^T) v, keys and values as the exact numbers they are stored as,
- *   scores, maximum, sum and products in fp32.  A query that sees no token: out 0, lse -inf.
+ *   out = softmax(scale q k^T) v, keys and values as the exact numbers they are stored as;
+ *   scores, maximum and sum in fp32, and a weight enters the product with the values, which is
+ *   summed in fp32, rounded to fp16 (2^-11).  A query that sees no token: out 0, lse -inf.  One
+ *   that sees a key that is not finite: both NaN; a value: out NaN, lse as without it.
  *   q        [T, Hq, D] fp16 or bf16 at the given strides; query head h reads cache head
  *            h / (Hq / H).
  *   tables   i32 [B, width]: the pages of each sequence, in order; tokens of a page outside

@@ -47,7 +47,8 @@ class Batch:
         self.v_words = flat[..., at + 4 * P:].view("<u4")
         self.tables = np.arange(self.B * self.per, dtype=np.int32).reshape(self.B, -1)
         T = sum(self.counts)
-        self.q = torch.randn(T, self.Hq, D, generator=torch.Generator().manual_seed(seed)).to(DT[dtype])
+        g = torch.Generator().manual_seed(seed)
+        self.q = torch.randn(T, self.Hq, D, generator=g).to(DT[dtype])
 
     def words(self, which, b, j):
         """The words [H] of sequence b's token j, as a view."""
@@ -252,7 +253,8 @@ def test_values_of_all_sizes(gpu, form, D):
 
 @every_form
 @pytest.mark.parametrize("dtype,size", [("fp16", 1.0), ("bf16", 1.0), ("bf16", 2.0 ** 20)])
-@pytest.mark.parametrize("factor", [2.0 ** 12, 2.0 ** 34, 2.0 ** 100, 2.0 ** -40, float("inf"), float("nan")])
+@pytest.mark.parametrize("factor", [2.0 ** 12, 2.0 ** 34, 2.0 ** 100, 2.0 ** -40, float("inf"),
+                                    float("nan")])
 def test_a_query_does_not_depend_on_the_others(gpu, form, dtype, size, factor):
     """One head of one query far larger or smaller than the rest, infinite or NaN: the other
     rows are what they are without it, bit for bit."""
@@ -314,7 +316,8 @@ def dirty(monkeypatch):
 
 
 @every_form
-@pytest.mark.parametrize("before,after,cut", [(0, 3, 0), (2, 0, 0), (5, 700, 0), (0, 0, 1), (1, 2, 2)])
+@pytest.mark.parametrize("before,after,cut", [(0, 3, 0), (2, 0, 0), (5, 700, 0), (0, 0, 1),
+                                              (1, 2, 2)])
 def test_rows_of_no_sequence_see_nothing(gpu, dirty, form, before, after, cut):
     """Rows before the first sequence's, after the last one's and past max_q: 0 and -inf."""
     x = Batch(form, "fp16", 64, L=140)
@@ -418,7 +421,8 @@ def test_a_bound_on_the_queries_far_above_them(gpu, form):
     (20000, 0, 6, 64, 16, 64, False, True, "fp16"),    # no queries: of 3, and of 2
     (33001, 2, 2, 128, 128, 0, False, True, "fp16"),   # all heads one after another
 ])
-def test_append_and_read_of_prompts_are_bit_exact(gpu, T, Hq, H, D, P, R, interleaved, rotate, dtype):
+def test_append_and_read_of_prompts_are_bit_exact(gpu, T, Hq, H, D, P, R, interleaved, rotate,
+                                                  dtype):
     """Enough tokens that a workgroup takes several heads one after another, from q to k to v."""
     g = torch.Generator().manual_seed(T + Hq)
     rows = torch.randn(T, Hq + 2 * H, D, generator=g)
@@ -435,7 +439,8 @@ def test_append_and_read_of_prompts_are_bit_exact(gpu, T, Hq, H, D, P, R, interl
         angle = torch.rand(500, R // 2, generator=g) * 6
         pos = torch.randint(0, 500, (T,), generator=g)
         c, s = angle.cos(), angle.sin()
-        turned = lambda x: oracle.turn(f32(x), c[pos].numpy(), s[pos].numpy(), interleaved)  # noqa: E731
+        cn, sn = c[pos].numpy(), s[pos].numpy()
+        turned = lambda x: oracle.turn(f32(x), cn, sn, interleaved)  # noqa: E731
         options = dict(positions=pos.to(gpu), cos=c.to(gpu), sin=s.to(gpu), interleaved=interleaved)
     cache = torch.full((pages, H, P, D + 8), 0xA5, dtype=torch.uint8, device=gpu)
     got = kv4.append(cache, on[:, :Hq] if Hq else None, on[:, Hq:Hq + H], on[:, Hq + H:], at,
