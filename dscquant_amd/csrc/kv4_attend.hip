@@ -140,7 +140,7 @@ struct Rows {
         for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(y[e]));
       }
       top = row_max(top);
-      if (top > 0.0f && top < INFINITY) k = min(15 - __builtin_amdgcn_frexp_expf(top), 60);
+      if (top > 0.0f && top < INFINITY) k = 15 - __builtin_amdgcn_frexp_expf(top);
     }
     to2 = __builtin_amdgcn_ldexpf(a.scale * kLog2e, -k);
 #pragma unroll

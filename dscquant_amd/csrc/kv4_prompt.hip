@@ -6,8 +6,8 @@
 // eight waves take 64 or 128 tokens in turn, a 16-token tile each, and leave keys and values
 // in LDS (twice, so that the next tokens are written while these are used), values as fp16 and
 // keys in the queries' type, which holds their whole numbers exactly and is then the queries'
-// own: every wave multiplies all of them with 32 rows of its own, as they are, which it holds
-// in registers.
+// own: every wave multiplies all of them with 32 rows of its own, which it holds in registers
+// as they are, but for a power of two.
 // 32 x 32 x 16 products: S^T (32 tokens x 32 rows) leaves lane (c, h) = (lane % 32, lane / 32)
 // the scores of row c and tokens 8 a + 4 h + i, which as they lie are the operand of
 // O^T += V^T P^T over the token order 16 s + 4 h + 0..3, 16 s + 8 + 4 h + 0..3; V^T is stored
@@ -64,6 +64,8 @@ struct Layout {
 template <typename T>
 struct Operand {
   typedef h8 V;
+  static constexpr float kRows = 1.0f;  // what rows are multiplied by
+  static __device__ __forceinline__ V rows(const Raw<T>& x) { return __builtin_bit_cast(V, x.w); }
   static __device__ __forceinline__ V of(const h2 e[4]) { return join8(e[0], e[1], e[2], e[3]); }
   static __device__ __forceinline__ f16 mfma(V a, V b, f16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
@@ -72,6 +74,16 @@ struct Operand {
 template <>
 struct Operand<bf16> {
   typedef __bf16 V __attribute__((ext_vector_type(8)));
+  // Products of the largest queries with D whole numbers stay within fp32 (2^127 2^-16 2^11).
+  static constexpr float kRows = 0x1p-16f;
+  static __device__ __forceinline__ V rows(const Raw<bf16>& x) {
+    float y[8];
+    to_f32(x, y);
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = pack_pair<bf16>(y[2 * i] * kRows, y[2 * i + 1] * kRows);
+    return __builtin_bit_cast(V, make_uint4(w[0], w[1], w[2], w[3]));
+  }
   static __device__ __forceinline__ V of(const h2 e[4]) {
     uint32_t w[4];
 #pragma unroll
@@ -354,8 +366,8 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_attend_prompt_kernel(KvAttend a
                   (head * G + min(row, count - 1) - i * G) * a.q_hs;
 #pragma unroll
   for (int ks = 0; ks < D / 16; ++ks)
-    w.q[ks] = __builtin_bit_cast(typename Operand<T>::V, load_raw_at<T>(qrow, 16 * ks + 8 * h).w);
-  const float to2 = a.scale * kLog2e;
+    w.q[ks] = Operand<T>::rows(load_raw_at<T>(qrow, 16 * ks + 8 * h));
+  const float to2 = a.scale * kLog2e / Operand<T>::kRows;
 
   const uint8_t* const block = a.cache.data + head * kv_block_bytes<D>(a.cache.P);
   const int64_t page_bytes = H * kv_block_bytes<D>(a.cache.P);

@@ -478,3 +478,17 @@ def test_the_least_scales(gpu, form, D):
     assert x.v_words.view("<f4").min() < 1e-8 and x.k_words.view("<f4").min() < 1e-8
     x.check(gpu, scale=2.0 ** 23 * D ** -0.5)
     x.check(gpu)  # scores of 0 or so
+
+
+@every_form
+@pytest.mark.parametrize("size", [2.0 ** -90, 2.0 ** 122])
+def test_queries_at_the_ends_of_their_range(gpu, form, size):
+    """A power of two that the scale undoes changes nothing, also beside a page that is not there."""
+    x = Batch(form, "bf16", 128)
+    x.tables = np.concatenate((x.tables[:, :1], np.full_like(x.tables[:, :1], -1), x.tables[:, 1:]), 1)
+    x.lengths = [n + x.P for n in x.lengths]
+    plain = x.run(gpu, scale=128 ** -0.5)
+    x.q *= size
+    have = x.run(gpu, scale=128 ** -0.5 / size)
+    for a, b in zip(have, plain):
+        assert np.isfinite(b).all() and np.array_equal(a, b)
